@@ -43,7 +43,7 @@ typedef enum {
 } mx_status;
 
 /* Element types. */
-enum { MX_DTYPE_F32 = 0, MX_DTYPE_F16 = 1, MX_DTYPE_I8 = 2, MX_DTYPE_I32 = 3, MX_DTYPE_U8 = 4 };
+enum { MX_DTYPE_F32 = 0, MX_DTYPE_F16 = 1, MX_DTYPE_I8 = 2, MX_DTYPE_I32 = 3, MX_DTYPE_U8 = 4, MX_DTYPE_BF16 = 5 };
 
 /* Packed numeric formats of the roundtrip probe (PackedNumericKernels.metal:35-96). */
 enum { MX_FMT_FP4_E2M1 = 0, MX_FMT_FP8_E4M3 = 1, MX_FMT_FP8_E5M2 = 2 };
@@ -94,7 +94,11 @@ enum {
    * codes with no widening; the f32 row scale is applied to the sums.  One
    * more launch (the split of x).  Hidden and intermediate % 64. */
   MX_WFMT_FP8_E4M3_F8X2 = 6,
-  MX_WFMT_FP8_E5M2_F8X2 = 7
+  MX_WFMT_FP8_E5M2_F8X2 = 7,
+  /* Block-scaled FP8: [N][K] E4M3 + f32 scales [ceil(N/128)][ceil(K/128)]
+   * (amax/448 of each 128 x 128 block); x and mid are quantized per row and
+   * 128 values (mx_block_quantize) and multiplied on the FP8 matrix cores. */
+  MX_WFMT_FP8_BLOCK = 8
 };
 
 /* MLPConfig (main.swift:62-66, MPPMLPKernels.metal:8-12). */
@@ -273,6 +277,79 @@ int mx_moe_benchmark(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, const
                      const void* x, const mx_mlp_weights* sets, int n_sets, void* out, int warmup,
                      int iterations, int use_graph, double* seconds_out);
 
+/* ---- MoE routing and exchange ------------------------------------------------- */
+/* No counterpart in the reference.  From gate logits to mx_moe_forward's rows
+ * and counts, and from its rows back to tokens.  All of it stays on the device
+ * in stream order; tokens = 0 is allowed and does nothing else than to clear
+ * the counts. */
+enum { MX_ROUTE_SOFTMAX = 0, MX_ROUTE_SIGMOID = 1 };
+typedef struct {
+  uint32_t tokens, experts, topk;   /* experts <= 512, topk <= 64 */
+  uint32_t score;                   /* MX_ROUTE_* */
+  /* groups > 1: the experts form that many runs of experts / groups, and only
+   * the topk_groups runs of the highest sum of their best group_top (1 or 2)
+   * keys are chosen from.  0 and 1: no groups. */
+  uint32_t groups, topk_groups, group_top; /* groups <= 64 */
+  uint32_t renormalize;             /* the chosen weights divided by their sum */
+  float scale;                      /* and multiplied by this */
+} mx_route_config;
+/* The topk experts of each token and their weights.
+ *   logits   [tokens] rows of `experts` f32, f16 or bf16 (logits_dtype),
+ *            logits_stride elements apart (0: experts).
+ *   bias     f32 [experts] or NULL.
+ *   ids      i32 [tokens][topk], weights f32 [tokens][topk].
+ * score p = softmax or 1/(1+exp(-logit)) in f32 (a softmax's sum in f64); key
+ * = p + bias.  The experts of the highest keys are taken in falling order,
+ * ties by the lowest index; weights are p, without the bias.  An expert whose
+ * logit is -inf or NaN, or whose key is, is not available; +inf counts as the
+ * largest float.  Slots that no available expert is left for get id -1 and
+ * weight 0. */
+int mx_moe_route(mx_ctx* ctx, const mx_route_config* cfg, const void* logits, int logits_dtype,
+                 size_t logits_stride, const float* bias, int32_t* ids, float* weights);
+/* Expert order of the (token, slot) pairs of ids i32 [tokens][topk]: by expert,
+ * then token, then slot.  counts i32 [experts] (<= 512) receives the rows of each
+ * expert, rows i32 [tokens][topk] the row of each pair, or -1 for ids outside
+ * [0, experts).  With xs, x [tokens][hidden] (f32, f16 or bf16) is copied into
+ * that order, xs [tokens * topk][hidden]; rows past the last pair are left as
+ * they are.  x and xs may both be NULL. */
+int mx_moe_dispatch(mx_ctx* ctx, int tokens, int topk, int experts, const int32_t* ids, int32_t* counts,
+                    int32_t* rows, const void* x, int dtype, int hidden, void* xs);
+/* out[t] = add[t] + sum over slots s of weights[t][s] * y[rows[t][s]], the
+ * products and sums in f32 and in the order of the slots; pairs of row -1
+ * contribute nothing, whatever their weight.  y [..][hidden] in y_dtype, add
+ * (or NULL) and out [tokens][hidden] in out_dtype (f32, f16, bf16).  add may
+ * be out. */
+int mx_moe_combine(mx_ctx* ctx, int tokens, int topk, int hidden, const void* y, int y_dtype,
+                   const int32_t* rows, const float* weights, const void* add, void* out, int out_dtype);
+
+/* ---- block-scaled FP8 ------------------------------------------------------------ */
+/* Activations to E4M3 with one f32 scale per row and 128 values: src [rows][k]
+ * (f32, f16, bf16) -> q [rows][k], scales [ceil(k/128)][rows].  scale =
+ * amax * (1/448 in f32), at least 2^-126, 1 where all 128 are zero; code =
+ * E4M3(x / scale), an f32 division, to nearest even.  128 values with a NaN or an infinity among them come out
+ * as NaN.  k % 16 == 0; rows = 0 is allowed. */
+int mx_block_quantize(mx_ctx* ctx, const void* src, int src_dtype, int rows, int k, uint8_t* q, float* scales);
+/* C[m][n] = sum over 128-blocks kb of a_scales[kb][m] * b_scales[n/128][kb] *
+ * sum_{k in kb} A[m][k] * B[n][k], with A as mx_block_quantize and B [n][k] as
+ * mx_fmt_quantize(MX_WFMT_FP8_BLOCK) writes them; f32 sums, C f32, f16 or
+ * bf16.  Any n >= 1, k % 16 == 0; m = 0 is allowed. */
+int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const uint8_t* b,
+                    const float* b_scales, void* c, int c_dtype, int m, int n, int k);
+/* The MLP of each token's experts with block-scaled FP8 weights, from token
+ * rows to token rows: dispatch, gate/up products, SwiGLU, down product and
+ * combine, with no host copy of ids or counts.
+ *   x        [tokens][hidden] f16 or bf16 (dtype), quantized as
+ *            mx_block_quantize does; so is the middle.
+ *   ids, weights  [tokens][topk] as mx_moe_route writes them.
+ *   w        experts stacked: gate and up data [E][I][H], down [E][H][I], each
+ *            with its experts' block scales one after the other.
+ *   add      [tokens][hidden] or NULL, added to the sum (a shared expert's rows).
+ *   out      [tokens][hidden] in dtype; may be add.
+ * 1 <= n_experts <= 512; hidden, intermediate % 16; cfg->tokens = 0 is allowed. */
+int mx_moe_block_forward(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, int topk, const void* x,
+                         int dtype, const int32_t* ids, const float* weights, const mx_mlp_weights* w,
+                         const void* add, void* out);
+
 /* ---- on-disk MXFP4 weights (safetensors) ------------------------------------- */
 /* Locate tensor `name` in a safetensors file (host only: no context, no
  * device).  dtype string (e.g. "U8"), shape (first max_dims entries), number
@@ -292,12 +369,13 @@ int mx_load_mxfp4(mx_ctx* ctx, const char* path, const char* blocks_name, const 
 
 /* ---- weight-format rows (config 3) ------------------------------------------ */
 /* Quantize f32 weights [rows][k] into format `wfmt` (scales per the enum;
- * the _F8X2 codes quantize as their FP8 format). */
+ * the _F8X2 codes quantize as their FP8 format).  k % 32; FP8_BLOCK k % 16. */
 int mx_fmt_quantize(mx_ctx* ctx, int wfmt, const float* w, int rows, int k, void* q,
                     void* scales);
 /* MLP with format weights: mpp_mlp_h_fp8e4m3_f_n128 / _h_fp8e5m2_f_n128 /
  * h_i8_f / h_i4_f / i8_i8_i32 rows (MPPMLPKernels.metal:50-125) with scales.
- * hidden and intermediate % 32; the _F8X2 rows % 64; W8A8 % 128. */
+ * hidden and intermediate % 32; the _F8X2 rows % 64; W8A8 % 128;
+ * FP8_BLOCK % 16. */
 int mx_fmt_mlp_forward(mx_ctx* ctx, int wfmt, const mx_mlp_config* cfg, const void* x,
                        const mx_mlp_weights* w, void* out);
 /* Timed loop of the format rows, as mx_mlp_benchmark (kernel_us_out and

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/mxfp4hip.h"
+#include "mx_block.h"
 #include "mx_internal.h"
 
 struct mx_ctx {
@@ -378,9 +379,14 @@ int run_steps(mx_ctx* c, const std::vector<Step>& steps) {
 
 }  // namespace
 
-// Context internals for the other translation units (mx_loader.cpp).
+// Context internals for the other translation units (mx_loader.cpp, mx_moe_api.cpp).
 hipStream_t mx_ctx_stream(mx_ctx* c) { return c->stream; }
 int mx_ctx_error(mx_ctx* c, int code, const char* message) { return set_err(c, code, "%s", message); }
+int mx_ctx_workspace(mx_ctx* c, size_t bytes, void** p) {
+  const int rc = ensure_ws(c, bytes);
+  *p = c->ws;
+  return rc;
+}
 
 // ===========================================================================
 extern "C" {
@@ -1019,9 +1025,14 @@ int mx_moe_benchmark(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, const i
 // ---- weight formats ---------------------------------------------------------------
 int mx_fmt_quantize(mx_ctx* c, int wfmt, const float* w, int rows, int k, void* q, void* scales) {
   if (!c) return MX_EINVAL;
-  if (rows <= 0 || k <= 0 || k % 32) return set_err(c, MX_EINVAL, "format quantize needs k % 32 == 0.");
+  if (rows <= 0 || k <= 0 || k % (wfmt == MX_WFMT_FP8_BLOCK ? 16 : 32))
+    return set_err(c, MX_EINVAL, "format quantize needs k %% 32 == 0 (block FP8: %% 16).");
   if (!w || !q || !scales || !aligned16(w) || !aligned16(q))
     return set_err(c, MX_EINVAL, "format quantize buffers must be non-null and 16-byte aligned.");
+  if (wfmt == MX_WFMT_FP8_BLOCK) {
+    MX_HIP(c, mx::launch_block_quantize_weights(w, rows, k, static_cast<uint8_t*>(q), static_cast<float*>(scales), c->stream));
+    return MX_OK;
+  }
   if (wfmt == MX_WFMT_FP8_E4M3_F8X2 || wfmt == MX_WFMT_FP8_E5M2_F8X2)
     wfmt = wfmt == MX_WFMT_FP8_E4M3_F8X2 ? MX_WFMT_FP8_E4M3 : MX_WFMT_FP8_E5M2;  // same weights
   switch (wfmt) {
@@ -1040,8 +1051,46 @@ int mx_fmt_quantize(mx_ctx* c, int wfmt, const float* w, int rows, int k, void* 
   return set_err(c, MX_EINVAL, "Unknown weight format %d.", wfmt);
 }
 
+// Block FP8: x and mid quantized per row and 128 values.
+static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x, const mx_mlp_weights* w, void* out,
+                             std::vector<Step>& steps) {
+  if (!cfg) return set_err(c, MX_EINVAL, "MLP config is null.");
+  if (cfg->tokens == 0 || cfg->hidden == 0 || cfg->intermediate == 0 || cfg->hidden % 16 || cfg->intermediate % 16)
+    return set_err(c, MX_EINVAL, "Block FP8 needs hidden and intermediate to be positive multiples of 16, and tokens.");
+  if (!x || !w || !out || !aligned16(x) || !aligned16(out))
+    return set_err(c, MX_EINVAL, "MLP buffers must be non-null and 16-byte aligned.");
+  const mx_qmatrix* mats[3] = {&w->gate, &w->up, &w->down};
+  for (const mx_qmatrix* m : mats)
+    if (!m->data || !m->scales || !aligned16(m->data) || (reinterpret_cast<uintptr_t>(m->scales) & 3u))
+      return set_err(c, MX_EINVAL, "format weight buffers must be non-null and 16-byte aligned.");
+  const int T = cfg->tokens, H = cfg->hidden, I = cfg->intermediate;
+  size_t off = 0;
+  auto take = [&](size_t bytes) { size_t o = off; off = align_up(off + bytes, 256); return o; };
+  const size_t bh = (H + mx::kQBlock - 1) / mx::kQBlock, bi = (I + mx::kQBlock - 1) / mx::kQBlock;
+  const size_t o_xq = take((size_t)T * H), o_xs = take(T * bh * 4), o_mid = take((size_t)T * I * 4),
+               o_mq = take((size_t)T * I), o_ms = take(T * bi * 4);
+  if (int rc = ensure_ws(c, off)) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(c->ws);
+  uint8_t *xq = ws + o_xq, *mq = ws + o_mq;
+  float *xs = reinterpret_cast<float*>(ws + o_xs), *mid = reinterpret_cast<float*>(ws + o_mid),
+        *ms = reinterpret_cast<float*>(ws + o_ms);
+  hipStream_t st = c->stream;
+  mx::BlockGemmArgs gu{}, dn{};
+  gu.a = xq; gu.a_s = xs; gu.a_rows = gu.m = T; gu.n = I; gu.k = H; gu.c = mid;
+  gu.w0 = static_cast<const uint8_t*>(w->gate.data); gu.s0 = static_cast<const float*>(w->gate.scales);
+  gu.w1 = static_cast<const uint8_t*>(w->up.data); gu.s1 = static_cast<const float*>(w->up.scales);
+  dn.a = mq; dn.a_s = ms; dn.a_rows = dn.m = T; dn.n = H; dn.k = I; dn.c = out;
+  dn.w0 = static_cast<const uint8_t*>(w->down.data); dn.s0 = static_cast<const float*>(w->down.scales);
+  steps.push_back({"block_quantize_x", [=] { return mx::launch_block_quantize(MX_DTYPE_F16, x, T, H, xq, xs, nullptr, st); }});
+  steps.push_back({"block_gemm_gate_up_swiglu", [=] { return mx::launch_block_gemm(MX_DTYPE_F32, gu, st); }});
+  steps.push_back({"block_quantize_mid", [=] { return mx::launch_block_quantize(MX_DTYPE_F32, mid, T, I, mq, ms, nullptr, st); }});
+  steps.push_back({"block_gemm_down", [=] { return mx::launch_block_gemm(MX_DTYPE_F16, dn, st); }});
+  return MX_OK;
+}
+
 static int build_fmt_steps(mx_ctx* c, int wfmt, const mx_mlp_config* cfg, const void* x,
                            const mx_mlp_weights* w, void* out, std::vector<Step>& steps) {
+  if (wfmt == MX_WFMT_FP8_BLOCK) return build_block_steps(c, cfg, x, w, out, steps);
   if (int rc = check_mlp_cfg(c, MX_MLP_FUSED, cfg)) return rc;
   if (!x || !w || !out) return set_err(c, MX_EINVAL, "MLP buffers must not be null.");
   int bk;
@@ -1160,7 +1209,9 @@ const char* mx_fmt_mlp_kernel_name(int wfmt, const mx_mlp_config* cfg, int index
   static const char* q[] = {"gemm_q_fmt_gate_up_swiglu", "gemm_q_fmt_down"};
   static const char* h[] = {"gemm_h_fmt_gate_up_swiglu", "gemm_h_fmt_down"};
   static const char* f8x2[] = {"split_x_f8x2", "gemm_q_f8x2_fmt_gate_up_swiglu", "gemm_q_f8x2_fmt_down"};
-  if (index < 0 || !cfg || wfmt < MX_WFMT_FP8_E4M3 || wfmt > MX_WFMT_FP8_E5M2_F8X2) return nullptr;
+  static const char* block[] = {"block_quantize_x", "block_gemm_gate_up_swiglu", "block_quantize_mid", "block_gemm_down"};
+  if (index < 0 || !cfg || wfmt < MX_WFMT_FP8_E4M3 || wfmt > MX_WFMT_FP8_BLOCK) return nullptr;
+  if (wfmt == MX_WFMT_FP8_BLOCK) return index < 4 ? block[index] : nullptr;
   if (wfmt == MX_WFMT_W8A8) return index < 4 ? w8a8[index] : nullptr;
   if (wfmt == MX_WFMT_FP8_E4M3_F8X2 || wfmt == MX_WFMT_FP8_E5M2_F8X2) return index < 3 ? f8x2[index] : nullptr;
   if (index >= 2) return nullptr;

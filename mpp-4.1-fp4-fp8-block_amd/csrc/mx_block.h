@@ -1,0 +1,87 @@
+// mx_block.h - launchers of the routed-experts operators (mx_moe.hip,
+// mx_block.hip), shared with the C-ABI layer.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/mxfp4hip.h"
+
+namespace mx {
+
+constexpr int kQBlock = 128;         // values (of weights: rows too) of one block scale
+constexpr int kMaxRouteExperts = 512;
+constexpr int kMaxRouteGroups = 64;
+
+// ---- router and exchange (mx_moe.hip) ---------------------------------------
+struct RouteArgs {
+  const void* logits;
+  size_t stride;                     // elements between the rows of logits
+  const float* bias;                 // null: none
+  int32_t* ids;
+  float* weights;
+  int tokens, experts, topk, groups, topk_groups, group_top;
+  int sigmoid, renormalize;
+  float scale;
+};
+hipError_t launch_route(int dtype, const RouteArgs& a, hipStream_t st);
+
+// A run of rows of one expert: one row tile of a grouped product.
+struct RowTile {
+  int expert, row0, rows, pad;
+};
+struct DispatchArgs {
+  const int32_t* ids;                // [tokens][topk]
+  int n, experts;                    // n = tokens topk slots
+  int32_t* counts;                   // [experts]
+  int32_t* rows;                     // [n] slot -> row, -1: none
+  int32_t* src;                      // [n] row -> slot; null: not wanted
+  RowTile* tiles;                    // row tiles of tile_rows rows; null: not wanted
+  int32_t* n_tiles;
+  int tile_rows;
+  int32_t* hist;                     // dispatch_ws_bytes
+};
+size_t dispatch_ws_bytes(int n, int experts);
+hipError_t launch_dispatch(const DispatchArgs& a, hipStream_t st);
+// xs[rows[t][s]] = x[t]; row_bytes of any size
+hipError_t launch_gather(const void* x, const int32_t* rows, void* xs, int tokens, int topk, size_t row_bytes,
+                         hipStream_t st);
+
+struct CombineArgs {
+  const void* y;
+  const int32_t* rows;
+  const float* weights;
+  const void* add;                   // null: none
+  void* out;
+  int tokens, topk, hidden;
+};
+hipError_t launch_combine(int y_dtype, int out_dtype, const CombineArgs& a, hipStream_t st);
+
+// ---- block-scaled FP8 (mx_block.hip) ------------------------------------------
+// n_rows: device count of the rows in use (null: all)
+hipError_t launch_block_quantize(int dtype, const void* src, int rows, int k, uint8_t* q, float* scales,
+                                 const int32_t* n_rows, hipStream_t st);
+hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_t* q, float* scales, hipStream_t st);
+
+// C[m][n] = sum_kb a_s[kb][m] w_s[n / 128][kb] sum_{k in kb} a[m][k] w[n][k], or with
+// w1 silu(C0) C1 of two such products.
+struct BlockGemmArgs {
+  const uint8_t* a;                  // E4M3 [a_rows][k]
+  const float* a_s;                  // [k / 128][a_rows]
+  int a_rows;
+  const uint8_t *w0, *w1;            // E4M3 [n][k]; w1 null: no SwiGLU
+  const float *s0, *s1;              // [n / 128][k / 128]
+  void* c;                           // [m][n]
+  int m, n, k;
+  // grouped: row tiles of experts, whose weights lie w_stride and s_stride apart
+  const RowTile* tiles;              // null: one matrix
+  const int32_t* n_tiles;
+  int max_tiles, tile_rows;
+  size_t w_stride, s_stride;
+  const int32_t* src;                // row -> slot, and
+  int src_div;                       // slot / src_div = row of a (null: row of a = row)
+};
+hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st);
+
+}  // namespace mx

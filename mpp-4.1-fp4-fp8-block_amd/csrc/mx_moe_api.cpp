@@ -1,0 +1,248 @@
+// mx_moe_api.cpp - C ABI of the routed-experts operators: router, dispatch,
+// combine, block-scaled FP8 (declared in include/mxfp4hip.h).
+#include <hip/hip_runtime.h>
+
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/mxfp4hip.h"
+#include "mx_block.h"
+
+// Context internals (mx_api.cpp).
+hipStream_t mx_ctx_stream(mx_ctx* c);
+int mx_ctx_error(mx_ctx* c, int code, const char* message);
+int mx_ctx_workspace(mx_ctx* c, size_t bytes, void** p);
+
+namespace {
+
+int fail(mx_ctx* c, int code, const char* fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return mx_ctx_error(c, code, buf);
+}
+
+#define MX_RUN(ctx, expr)                                                                           \
+  do {                                                                                              \
+    const hipError_t e_ = (expr);                                                                   \
+    if (e_ != hipSuccess) return fail(ctx, MX_EGPU, "%s failed: %s", #expr, hipGetErrorString(e_)); \
+  } while (0)
+
+bool is_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool is_float(int dtype) { return dtype == MX_DTYPE_F32 || dtype == MX_DTYPE_F16 || dtype == MX_DTYPE_BF16; }
+size_t size_of(int dtype) { return dtype == MX_DTYPE_F32 ? 4 : 2; }
+int blocks(int n) { return (n + mx::kQBlock - 1) / mx::kQBlock; }
+
+// slots of a batch: tokens and pairs have to be counted in 31 bits
+int check_slots(mx_ctx* c, int tokens, int topk) {
+  if (tokens < 0 || topk < 1 || topk > 64) return fail(c, MX_EINVAL, "MoE needs tokens >= 0 and topk in 1..64.");
+  if ((long long)tokens * topk > 0x3fffffff) return fail(c, MX_EINVAL, "MoE tokens x topk must be below 2^30.");
+  return MX_OK;
+}
+
+int check_experts(mx_ctx* c, int experts) {
+  if (experts < 1 || experts > mx::kMaxRouteExperts)
+    return fail(c, MX_EINVAL, "MoE routing needs 1 to %d experts.", mx::kMaxRouteExperts);
+  return MX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mx_moe_route(mx_ctx* c, const mx_route_config* cfg, const void* logits, int logits_dtype, size_t logits_stride,
+                 const float* bias, int32_t* ids, float* weights) {
+  if (!c) return MX_EINVAL;
+  if (!cfg) return fail(c, MX_EINVAL, "route config is null.");
+  if (cfg->tokens > 0x7fffffffu || cfg->experts > 0x7fffffffu || cfg->topk > 64)
+    return fail(c, MX_EINVAL, "route sizes are out of range.");
+  const int T = (int)cfg->tokens, E = (int)cfg->experts, K = (int)cfg->topk;
+  if (int rc = check_slots(c, T, K)) return rc;
+  if (int rc = check_experts(c, E)) return rc;
+  if (K > E) return fail(c, MX_EINVAL, "route topk %d is more than %d experts.", K, E);
+  if (cfg->score != MX_ROUTE_SOFTMAX && cfg->score != MX_ROUTE_SIGMOID)
+    return fail(c, MX_EINVAL, "Unknown route score %u.", cfg->score);
+  if (!is_float(logits_dtype)) return fail(c, MX_EINVAL, "route logits must be f32, f16 or bf16.");
+  const int G = cfg->groups > 1 ? (int)cfg->groups : 1;
+  if (cfg->groups > (uint32_t)mx::kMaxRouteGroups || E % G)
+    return fail(c, MX_EINVAL, "route groups must divide the experts and be at most %d.", mx::kMaxRouteGroups);
+  if (G > 1) {
+    if (cfg->topk_groups < 1 || cfg->topk_groups > (uint32_t)G)
+      return fail(c, MX_EINVAL, "route topk_groups must be 1 to %d.", G);
+    if (cfg->group_top != 1 && cfg->group_top != 2) return fail(c, MX_EINVAL, "route group_top must be 1 or 2.");
+    if ((long)cfg->topk_groups * (E / G) < K)
+      return fail(c, MX_EINVAL, "route topk is more than the experts of topk_groups groups.");
+  }
+  if (logits_stride && logits_stride < (size_t)E) return fail(c, MX_EINVAL, "route logits_stride is below the experts.");
+  if (T == 0) return MX_OK;
+  if (!logits || !ids || !weights) return fail(c, MX_EINVAL, "route buffers must not be null.");
+  if (!is_aligned(logits, size_of(logits_dtype)) || !is_aligned(bias, 4) || !is_aligned(ids, 4) || !is_aligned(weights, 4))
+    return fail(c, MX_EINVAL, "route buffers must be aligned to their elements.");
+  const mx::RouteArgs a{logits, logits_stride ? logits_stride : (size_t)E, bias, ids, weights, T, E, K, G,
+                        (int)cfg->topk_groups, (int)cfg->group_top, cfg->score == MX_ROUTE_SIGMOID,
+                        cfg->renormalize != 0, cfg->scale};
+  MX_RUN(c, mx::launch_route(logits_dtype, a, mx_ctx_stream(c)));
+  return MX_OK;
+}
+
+int mx_moe_dispatch(mx_ctx* c, int tokens, int topk, int experts, const int32_t* ids, int32_t* counts, int32_t* rows,
+                    const void* x, int dtype, int hidden, void* xs) {
+  if (!c) return MX_EINVAL;
+  if (int rc = check_slots(c, tokens, topk)) return rc;
+  if (int rc = check_experts(c, experts)) return rc;
+  if (!counts || (tokens && (!ids || !rows))) return fail(c, MX_EINVAL, "dispatch buffers must not be null.");
+  if (!is_aligned(ids, 4) || !is_aligned(counts, 4) || !is_aligned(rows, 4))
+    return fail(c, MX_EINVAL, "dispatch ids, counts and rows must be 4-byte aligned.");
+  if (!x != !xs) return fail(c, MX_EINVAL, "dispatch takes both x and xs or neither.");
+  if (x) {
+    if (!is_float(dtype)) return fail(c, MX_EINVAL, "dispatch rows must be f32, f16 or bf16.");
+    if (hidden < 1) return fail(c, MX_EINVAL, "dispatch hidden must be positive.");
+    if (!is_aligned(x, size_of(dtype)) || !is_aligned(xs, size_of(dtype)))
+      return fail(c, MX_EINVAL, "dispatch rows must be aligned to their elements.");
+  }
+  const int n = tokens * topk;
+  void* ws = nullptr;
+  if (int rc = mx_ctx_workspace(c, mx::dispatch_ws_bytes(n, experts), &ws)) return rc;
+  mx::DispatchArgs a{};
+  a.ids = ids;
+  a.n = n;
+  a.experts = experts;
+  a.counts = counts;
+  a.rows = rows;
+  a.hist = static_cast<int32_t*>(ws);
+  MX_RUN(c, mx::launch_dispatch(a, mx_ctx_stream(c)));
+  if (x && tokens)
+    MX_RUN(c, mx::launch_gather(x, rows, xs, tokens, topk, (size_t)hidden * size_of(dtype), mx_ctx_stream(c)));
+  return MX_OK;
+}
+
+int mx_moe_combine(mx_ctx* c, int tokens, int topk, int hidden, const void* y, int y_dtype, const int32_t* rows,
+                   const float* weights, const void* add, void* out, int out_dtype) {
+  if (!c) return MX_EINVAL;
+  if (int rc = check_slots(c, tokens, topk)) return rc;
+  if (hidden < 1) return fail(c, MX_EINVAL, "combine hidden must be positive.");
+  if (!is_float(y_dtype) || !is_float(out_dtype)) return fail(c, MX_EINVAL, "combine rows must be f32, f16 or bf16.");
+  if (tokens == 0) return MX_OK;
+  if (!y || !rows || !weights || !out) return fail(c, MX_EINVAL, "combine buffers must not be null.");
+  if (!is_aligned(y, size_of(y_dtype)) || !is_aligned(add, size_of(out_dtype)) || !is_aligned(out, size_of(out_dtype)) ||
+      !is_aligned(rows, 4) || !is_aligned(weights, 4))
+    return fail(c, MX_EINVAL, "combine buffers must be aligned to their elements.");
+  const mx::CombineArgs a{y, rows, weights, add, out, tokens, topk, hidden};
+  MX_RUN(c, mx::launch_combine(y_dtype, out_dtype, a, mx_ctx_stream(c)));
+  return MX_OK;
+}
+
+int mx_block_quantize(mx_ctx* c, const void* src, int src_dtype, int rows, int k, uint8_t* q, float* scales) {
+  if (!c) return MX_EINVAL;
+  if (rows < 0 || k <= 0 || k % 16) return fail(c, MX_EINVAL, "block quantize needs rows >= 0 and k a positive multiple of 16.");
+  if (!is_float(src_dtype)) return fail(c, MX_EINVAL, "block quantize source must be f32, f16 or bf16.");
+  if (rows == 0) return MX_OK;
+  if (!src || !q || !scales || !is_aligned(src, 16) || !is_aligned(q, 16) || !is_aligned(scales, 4))
+    return fail(c, MX_EINVAL, "block quantize buffers must be non-null, source and codes 16-byte and scales 4-byte aligned.");
+  MX_RUN(c, mx::launch_block_quantize(src_dtype, src, rows, k, q, scales, nullptr, mx_ctx_stream(c)));
+  return MX_OK;
+}
+
+int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const uint8_t* b, const float* b_scales, void* out,
+                    int c_dtype, int m, int n, int k) {
+  if (!c) return MX_EINVAL;
+  if (m < 0 || n <= 0 || k <= 0 || k % 16)
+    return fail(c, MX_EINVAL, "block matmul needs m >= 0, n > 0 and k a positive multiple of 16.");
+  if (!is_float(c_dtype)) return fail(c, MX_EINVAL, "block matmul C must be f32, f16 or bf16.");
+  if (m == 0) return MX_OK;
+  if (!a || !a_scales || !b || !b_scales || !out || !is_aligned(a, 16) || !is_aligned(b, 16) || !is_aligned(out, 16) ||
+      !is_aligned(a_scales, 4) || !is_aligned(b_scales, 4))
+    return fail(c, MX_EINVAL, "block matmul buffers must be non-null, codes and C 16-byte and scales 4-byte aligned.");
+  mx::BlockGemmArgs g{};
+  g.a = a;
+  g.a_s = a_scales;
+  g.a_rows = m;
+  g.w0 = b;
+  g.s0 = b_scales;
+  g.c = out;
+  g.m = m;
+  g.n = n;
+  g.k = k;
+  MX_RUN(c, mx::launch_block_gemm(c_dtype, g, mx_ctx_stream(c)));
+  return MX_OK;
+}
+
+int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int topk, const void* x, int dtype,
+                         const int32_t* ids, const float* weights, const mx_mlp_weights* w, const void* add, void* out) {
+  if (!c) return MX_EINVAL;
+  if (!cfg) return fail(c, MX_EINVAL, "MLP config is null.");
+  if (cfg->tokens > 0x7fffffffu || cfg->hidden > 0x7ffffff0u || cfg->intermediate > 0x7ffffff0u)
+    return fail(c, MX_EINVAL, "MLP sizes are out of range.");
+  const int T = (int)cfg->tokens, H = (int)cfg->hidden, I = (int)cfg->intermediate, E = n_experts;
+  if (int rc = check_slots(c, T, topk)) return rc;
+  if (int rc = check_experts(c, E)) return rc;
+  if (H < 16 || I < 16 || H % 16 || I % 16)
+    return fail(c, MX_EINVAL, "Block FP8 needs hidden and intermediate to be positive multiples of 16.");
+  if (dtype != MX_DTYPE_F16 && dtype != MX_DTYPE_BF16) return fail(c, MX_EINVAL, "MoE rows must be f16 or bf16.");
+  if (!w) return fail(c, MX_EINVAL, "MLP weight buffers must not be null.");
+  const mx_qmatrix* mats[3] = {&w->gate, &w->up, &w->down};
+  for (const mx_qmatrix* m : mats)
+    if (!m->data || !m->scales || !is_aligned(m->data, 16) || !is_aligned(m->scales, 4))
+      return fail(c, MX_EINVAL, "Block FP8 weights must be non-null, codes 16-byte and scales 4-byte aligned.");
+  if (T == 0) return MX_OK;
+  if (!x || !ids || !weights || !out) return fail(c, MX_EINVAL, "MoE buffers must not be null.");
+  if (!is_aligned(x, 16) || !is_aligned(out, 16) || !is_aligned(add, 16) || !is_aligned(ids, 4) || !is_aligned(weights, 4))
+    return fail(c, MX_EINVAL, "MoE rows must be 16-byte aligned, ids and weights 4-byte.");
+  const int n = T * topk;
+  size_t off = 0;
+  auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
+  const int tile_rows = 64, max_tiles = (n < E ? n : E) + n / tile_rows;
+  const size_t o_xq = take((size_t)T * H), o_xs = take((size_t)T * blocks(H) * 4), o_rows = take((size_t)n * 4),
+               o_src = take((size_t)n * 4), o_counts = take((size_t)E * 4), o_tiles = take((size_t)max_tiles * sizeof(mx::RowTile)),
+               o_nt = take(4), o_hist = take(mx::dispatch_ws_bytes(n, E)), o_mid = take((size_t)n * I * 4),
+               o_mq = take((size_t)n * I), o_ms = take((size_t)n * blocks(I) * 4), o_y = take((size_t)n * H * 4);
+  void* p = nullptr;
+  if (int rc = mx_ctx_workspace(c, off, &p)) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(p);
+  hipStream_t st = mx_ctx_stream(c);
+  mx::DispatchArgs d{ids, n, E, reinterpret_cast<int32_t*>(ws + o_counts), reinterpret_cast<int32_t*>(ws + o_rows),
+                     reinterpret_cast<int32_t*>(ws + o_src), reinterpret_cast<mx::RowTile*>(ws + o_tiles),
+                     reinterpret_cast<int32_t*>(ws + o_nt), tile_rows, reinterpret_cast<int32_t*>(ws + o_hist)};
+  MX_RUN(c, mx::launch_dispatch(d, st));
+  MX_RUN(c, mx::launch_block_quantize(dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), nullptr, st));
+  mx::BlockGemmArgs g{};
+  g.a = ws + o_xq;
+  g.a_s = reinterpret_cast<float*>(ws + o_xs);
+  g.a_rows = T;
+  g.w0 = static_cast<const uint8_t*>(w->gate.data);
+  g.w1 = static_cast<const uint8_t*>(w->up.data);
+  g.s0 = static_cast<const float*>(w->gate.scales);
+  g.s1 = static_cast<const float*>(w->up.scales);
+  g.c = ws + o_mid;
+  g.m = n;
+  g.n = I;
+  g.k = H;
+  g.tiles = d.tiles;
+  g.n_tiles = d.n_tiles;
+  g.max_tiles = max_tiles;
+  g.tile_rows = tile_rows;
+  g.w_stride = (size_t)I * H;
+  g.s_stride = (size_t)blocks(I) * blocks(H);
+  g.src = d.src;
+  g.src_div = topk;
+  MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
+  MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + o_mid, n, I, ws + o_mq, reinterpret_cast<float*>(ws + o_ms), nullptr, st));
+  g.a = ws + o_mq;
+  g.a_s = reinterpret_cast<float*>(ws + o_ms);
+  g.a_rows = n;
+  g.w0 = static_cast<const uint8_t*>(w->down.data);
+  g.w1 = nullptr;
+  g.s0 = static_cast<const float*>(w->down.scales);
+  g.c = ws + o_y;
+  g.n = H;
+  g.k = I;
+  g.src = nullptr;
+  MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
+  const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H};
+  MX_RUN(c, mx::launch_combine(MX_DTYPE_F32, dtype, b, st));
+  return MX_OK;
+}
+
+}  // extern "C"

@@ -15,12 +15,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libmxfp4hip.so")
 
 MX_OK, MX_EINVAL, MX_ENODEV, MX_ENOKERNEL, MX_ENOMEM, MX_EGPU = range(6)
-DT_F32, DT_F16, DT_I8, DT_I32, DT_U8 = range(5)
+DT_F32, DT_F16, DT_I8, DT_I32, DT_U8, DT_BF16 = range(6)
 FMT_FP4_E2M1, FMT_FP8_E4M3, FMT_FP8_E5M2 = range(3)
 MLP_FUSED, MLP_DEQUANT, MLP_W4A4, MLP_REFROW, MLP_SCALED = range(5)
 PROBE_F16, PROBE_FP4, PROBE_FP8, PROBE_INT4, PROBE_I8 = range(5)
 WFMT_FP8_E4M3, WFMT_FP8_E5M2, WFMT_INT8, WFMT_INT4, WFMT_W8A8 = 1, 2, 3, 4, 5
 WFMT_FP8_E4M3_F8X2, WFMT_FP8_E5M2_F8X2 = 6, 7  # FP8 weights on the scaled FP8 MFMA (F8X2 activations)
+WFMT_FP8_BLOCK = 8  # E4M3 with one f32 scale per 128 x 128 weights
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
 # Every symbol the header declares (checked by tests/test_abi_exports.py).
 EXPORTS = [
@@ -29,6 +31,7 @@ EXPORTS = [
     "mx_download", "mx_memset", "mx_roundtrip", "mx_pack", "mx_unpack", "mx_mxfp4_quantize",
     "mx_mxfp4_dequant_f16", "mx_mxfp4_matmul", "mx_gemm_f16", "mx_gemm_i8", "mx_accum_gemm", "mx_swiglu", "mx_mlp_forward",
     "mx_mlp_benchmark", "mx_mlp_kernel_name", "mx_mlp_forward_noalloc", "mx_moe_forward", "mx_moe_benchmark",
+    "mx_moe_route", "mx_moe_dispatch", "mx_moe_combine", "mx_block_quantize", "mx_block_matmul", "mx_moe_block_forward",
     "mx_safetensors_find", "mx_load_mxfp4",
     "mx_fmt_quantize", "mx_fmt_mlp_forward",
     "mx_fmt_mlp_benchmark", "mx_fmt_mlp_kernel_name", "mx_fill_normal", "mx_lcg_bytes", "mx_lcg_pattern", "mx_lcg_half",
@@ -68,6 +71,11 @@ class QMatrix(ctypes.Structure):
 
 class MlpWeights(ctypes.Structure):
     _fields_ = [("gate", QMatrix), ("up", QMatrix), ("down", QMatrix)]
+
+
+class RouteConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("tokens", "experts", "topk", "score", "groups", "topk_groups",
+                                               "group_top", "renormalize")] + [("scale", ctypes.c_float)]
 
 
 _vp, _sz, _int, _u32, _u64, _f = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32,
@@ -117,6 +125,12 @@ def load() -> ctypes.CDLL:
                                     _int, _int, P(ctypes.c_double), P(ctypes.c_double), P(_int)]),
         "mx_mlp_kernel_name": (ctypes.c_char_p, [_int, ctypes.c_void_p, _int]),
         "mx_moe_forward": (_int, [_vp, P(MlpConfig), _int, P(_int), _vp, P(MlpWeights), _vp]),
+        "mx_moe_route": (_int, [_vp, P(RouteConfig), _vp, _int, _sz, _vp, _vp, _vp]),
+        "mx_moe_dispatch": (_int, [_vp, _int, _int, _int, _vp, _vp, _vp, _vp, _int, _int, _vp]),
+        "mx_moe_combine": (_int, [_vp, _int, _int, _int, _vp, _int, _vp, _vp, _vp, _vp, _int]),
+        "mx_block_quantize": (_int, [_vp, _vp, _int, _int, _int, _vp, _vp]),
+        "mx_block_matmul": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int]),
+        "mx_moe_block_forward": (_int, [_vp, P(MlpConfig), _int, _int, _vp, _int, _vp, _vp, P(MlpWeights), _vp, _vp]),
         "mx_safetensors_find": (_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _sz,
                                        P(ctypes.c_longlong), _int, P(_int), P(ctypes.c_ulonglong),
                                        P(ctypes.c_ulonglong)]),
@@ -352,6 +366,41 @@ class Device:
                                             len(sets), out.p, warmup, iterations, 1 if graph else 0,
                                             ctypes.byref(secs)))
         return secs.value
+
+    # ---- MoE routing and exchange, block-scaled FP8 ----
+    def moe_route(self, tokens, experts, topk, logits: DevBuf, logits_dtype, ids: DevBuf, weights: DevBuf, bias=None,
+                  score=ROUTE_SOFTMAX, groups=1, topk_groups=1, group_top=1, renormalize=False, scale=1.0, stride=0):
+        """Top experts of each token and their weights (mx_moe_route)."""
+        cfg = RouteConfig(tokens, experts, topk, score, groups, topk_groups, group_top, bool(renormalize), scale)
+        self._check(load().mx_moe_route(self.ctx, ctypes.byref(cfg), logits.p, logits_dtype, stride, bias and bias.p,
+                                        ids.p, weights.p))
+
+    def moe_dispatch(self, tokens, topk, experts, ids: DevBuf, counts: DevBuf, rows: DevBuf, x=None, dtype=DT_F16,
+                     hidden=0, xs=None):
+        """Counts and rows of the expert order, and x in it (mx_moe_dispatch)."""
+        self._check(load().mx_moe_dispatch(self.ctx, tokens, topk, experts, ids.p, counts.p, rows.p, x and x.p, dtype,
+                                           hidden, xs and xs.p))
+
+    def moe_combine(self, tokens, topk, hidden, y: DevBuf, y_dtype, rows: DevBuf, weights: DevBuf, out: DevBuf, out_dtype,
+                    add=None):
+        """Weighted sums of the experts' rows, in token order (mx_moe_combine)."""
+        self._check(load().mx_moe_combine(self.ctx, tokens, topk, hidden, y.p, y_dtype, rows.p, weights.p, add and add.p,
+                                          out.p, out_dtype))
+
+    def block_quantize(self, src: DevBuf, src_dtype, rows, k, q: DevBuf, scales: DevBuf):
+        """Activations to E4M3 with a scale per row and 128 values (mx_block_quantize)."""
+        self._check(load().mx_block_quantize(self.ctx, src.p, src_dtype, rows, k, q.p, scales.p))
+
+    def block_matmul(self, a: DevBuf, a_scales: DevBuf, b: DevBuf, b_scales: DevBuf, c: DevBuf, c_dtype, m, n, k):
+        """Product of block-scaled FP8 matrices (mx_block_matmul)."""
+        self._check(load().mx_block_matmul(self.ctx, a.p, a_scales.p, b.p, b_scales.p, c.p, c_dtype, m, n, k))
+
+    def moe_block_forward(self, tokens, hidden, inter, experts, topk, x: DevBuf, dtype, ids: DevBuf, weights: DevBuf,
+                          w: MlpWeights, out: DevBuf, add=None):
+        """The MLP of each token's block-FP8 experts (mx_moe_block_forward)."""
+        cfg = MlpConfig(tokens, hidden, inter)
+        self._check(load().mx_moe_block_forward(self.ctx, ctypes.byref(cfg), experts, topk, x.p, dtype, ids.p, weights.p,
+                                                ctypes.byref(w), add and add.p, out.p))
 
     def fmt_quantize(self, wfmt, w: DevBuf, rows, k, q: DevBuf, scales: DevBuf):
         self._check(load().mx_fmt_quantize(self.ctx, wfmt, w.p, rows, k, q.p, scales.p))
