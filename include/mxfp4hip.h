@@ -332,7 +332,7 @@ int mx_block_quantize(mx_ctx* ctx, const void* src, int src_dtype, int rows, int
 /* C[m][n] = sum over 128-blocks kb of a_scales[kb][m] * b_scales[n/128][kb] *
  * sum_{k in kb} A[m][k] * B[n][k], with A as mx_block_quantize and B [n][k] as
  * mx_fmt_quantize(MX_WFMT_FP8_BLOCK) writes them; f32 sums, C f32, f16 or
- * bf16.  Any n >= 1, k % 16 == 0; m = 0 is allowed. */
+ * bf16.  Any n >= 1, k % 16 == 0, k <= 65536; m = 0 is allowed. */
 int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const uint8_t* b,
                     const float* b_scales, void* c, int c_dtype, int m, int n, int k);
 /* The MLP of each token's experts with block-scaled FP8 weights, from token
@@ -345,7 +345,8 @@ int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const 
  *            with its experts' block scales one after the other.
  *   add      [tokens][hidden] or NULL, added to the sum (a shared expert's rows).
  *   out      [tokens][hidden] in dtype; may be add.
- * 1 <= n_experts <= 512; hidden, intermediate % 16; cfg->tokens = 0 is allowed. */
+ * 1 <= n_experts <= 512; hidden, intermediate % 16 and <= 65536; cfg->tokens = 0 is
+ * allowed. */
 int mx_moe_block_forward(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, int topk, const void* x,
                          int dtype, const int32_t* ids, const float* weights, const mx_mlp_weights* w,
                          const void* add, void* out);

@@ -1057,6 +1057,9 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
   if (!cfg) return set_err(c, MX_EINVAL, "MLP config is null.");
   if (cfg->tokens == 0 || cfg->hidden == 0 || cfg->intermediate == 0 || cfg->hidden % 16 || cfg->intermediate % 16)
     return set_err(c, MX_EINVAL, "Block FP8 needs hidden and intermediate to be positive multiples of 16, and tokens.");
+  constexpr uint32_t kMost = mx::kMaxBlocks * mx::kQBlock;
+  if (cfg->tokens > 0x7fffffffu || cfg->hidden > kMost || cfg->intermediate > kMost)
+    return set_err(c, MX_EINVAL, "Block FP8 hidden and intermediate are at most %u.", kMost);
   if (!x || !w || !out || !aligned16(x) || !aligned16(out))
     return set_err(c, MX_EINVAL, "MLP buffers must be non-null and 16-byte aligned.");
   const mx_qmatrix* mats[3] = {&w->gate, &w->up, &w->down};
@@ -1067,7 +1070,9 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
   size_t off = 0;
   auto take = [&](size_t bytes) { size_t o = off; off = align_up(off + bytes, 256); return o; };
   const size_t bh = (H + mx::kQBlock - 1) / mx::kQBlock, bi = (I + mx::kQBlock - 1) / mx::kQBlock;
-  const size_t o_xq = take((size_t)T * H), o_xs = take(T * bh * 4), o_mid = take((size_t)T * I * 4),
+  const int gu_rows = mx::block_tile_rows(T, 1, I, MX_DTYPE_F32, true);
+  const bool few = gu_rows == 16;  // the middle comes in f32; else in its codes
+  const size_t o_xq = take((size_t)T * H), o_xs = take(T * bh * 4), o_mid = take(few ? (size_t)T * I * 4 : 0),
                o_mq = take((size_t)T * I), o_ms = take(T * bi * 4);
   if (int rc = ensure_ws(c, off)) return rc;
   uint8_t* ws = static_cast<uint8_t*>(c->ws);
@@ -1076,14 +1081,15 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
         *ms = reinterpret_cast<float*>(ws + o_ms);
   hipStream_t st = c->stream;
   mx::BlockGemmArgs gu{}, dn{};
-  gu.a = xq; gu.a_s = xs; gu.a_rows = gu.m = T; gu.n = I; gu.k = H; gu.c = mid;
+  gu.a = xq; gu.a_s = xs; gu.a_rows = gu.m = T; gu.n = I; gu.k = H; gu.tile_rows = gu_rows;
+  gu.c = few ? static_cast<void*>(mid) : mq; gu.c_s = ms;
   gu.w0 = static_cast<const uint8_t*>(w->gate.data); gu.s0 = static_cast<const float*>(w->gate.scales);
   gu.w1 = static_cast<const uint8_t*>(w->up.data); gu.s1 = static_cast<const float*>(w->up.scales);
-  dn.a = mq; dn.a_s = ms; dn.a_rows = dn.m = T; dn.n = H; dn.k = I; dn.c = out;
+  dn.a = mq; dn.a_s = ms; dn.a_rows = dn.m = T; dn.n = H; dn.k = I; dn.c = out; dn.tile_rows = mx::block_tile_rows(T, 1, H, MX_DTYPE_F16, false);
   dn.w0 = static_cast<const uint8_t*>(w->down.data); dn.s0 = static_cast<const float*>(w->down.scales);
-  steps.push_back({"block_quantize_x", [=] { return mx::launch_block_quantize(MX_DTYPE_F16, x, T, H, xq, xs, nullptr, st); }});
-  steps.push_back({"block_gemm_gate_up_swiglu", [=] { return mx::launch_block_gemm(MX_DTYPE_F32, gu, st); }});
-  steps.push_back({"block_quantize_mid", [=] { return mx::launch_block_quantize(MX_DTYPE_F32, mid, T, I, mq, ms, nullptr, st); }});
+  steps.push_back({"block_quantize_x", [=] { return mx::launch_block_quantize(MX_DTYPE_F16, x, T, H, xq, xs, st); }});
+  steps.push_back({mx_fmt_mlp_kernel_name(MX_WFMT_FP8_BLOCK, cfg, 1), [=] { return mx::launch_block_gemm(MX_DTYPE_F32, gu, st); }});
+  if (few) steps.push_back({"block_quantize_mid", [=] { return mx::launch_block_quantize(MX_DTYPE_F32, mid, T, I, mq, ms, st); }});
   steps.push_back({"block_gemm_down", [=] { return mx::launch_block_gemm(MX_DTYPE_F16, dn, st); }});
   return MX_OK;
 }
@@ -1210,8 +1216,12 @@ const char* mx_fmt_mlp_kernel_name(int wfmt, const mx_mlp_config* cfg, int index
   static const char* h[] = {"gemm_h_fmt_gate_up_swiglu", "gemm_h_fmt_down"};
   static const char* f8x2[] = {"split_x_f8x2", "gemm_q_f8x2_fmt_gate_up_swiglu", "gemm_q_f8x2_fmt_down"};
   static const char* block[] = {"block_quantize_x", "block_gemm_gate_up_swiglu", "block_quantize_mid", "block_gemm_down"};
+  static const char* block3[] = {"block_quantize_x", "block_gemm_gate_up_swiglu_quantize", "block_gemm_down"};
   if (index < 0 || !cfg || wfmt < MX_WFMT_FP8_E4M3 || wfmt > MX_WFMT_FP8_BLOCK) return nullptr;
-  if (wfmt == MX_WFMT_FP8_BLOCK) return index < 4 ? block[index] : nullptr;
+  if (wfmt == MX_WFMT_FP8_BLOCK) {
+    if (mx::block_tile_rows(cfg->tokens, 1, cfg->intermediate, MX_DTYPE_F32, true) == 16) return index < 4 ? block[index] : nullptr;
+    return index < 3 ? block3[index] : nullptr;
+  }
   if (wfmt == MX_WFMT_W8A8) return index < 4 ? w8a8[index] : nullptr;
   if (wfmt == MX_WFMT_FP8_E4M3_F8X2 || wfmt == MX_WFMT_FP8_E5M2_F8X2) return index < 3 ? f8x2[index] : nullptr;
   if (index >= 2) return nullptr;

@@ -11,6 +11,7 @@
 namespace mx {
 
 constexpr int kQBlock = 128;         // values (of weights: rows too) of one block scale
+constexpr int kMaxBlocks = 512;       // blocks of K in one product
 constexpr int kMaxRouteExperts = 512;
 constexpr int kMaxRouteGroups = 64;
 
@@ -59,9 +60,8 @@ struct CombineArgs {
 hipError_t launch_combine(int y_dtype, int out_dtype, const CombineArgs& a, hipStream_t st);
 
 // ---- block-scaled FP8 (mx_block.hip) ------------------------------------------
-// n_rows: device count of the rows in use (null: all)
 hipError_t launch_block_quantize(int dtype, const void* src, int rows, int k, uint8_t* q, float* scales,
-                                 const int32_t* n_rows, hipStream_t st);
+                                 hipStream_t st);
 hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_t* q, float* scales, hipStream_t st);
 
 // C[m][n] = sum_kb a_s[kb][m] w_s[n / 128][kb] sum_{k in kb} a[m][k] w[n][k], or with
@@ -72,16 +72,25 @@ struct BlockGemmArgs {
   int a_rows;
   const uint8_t *w0, *w1;            // E4M3 [n][k]; w1 null: no SwiGLU
   const float *s0, *s1;              // [n / 128][k / 128]
-  void* c;                           // [m][n]
+  void* c;                           // [m][n]; SwiGLU: E4M3 codes, and
+  float* c_s;                        // their scales [n / 128][m]
   int m, n, k;
+  int tile_rows;                     // block_tile_rows
   // grouped: row tiles of experts, whose weights lie w_stride and s_stride apart
   const RowTile* tiles;              // null: one matrix
   const int32_t* n_tiles;
-  int max_tiles, tile_rows;
+  int max_tiles;
   size_t w_stride, s_stride;
   const int32_t* src;                // row -> slot, and
   int src_div;                       // slot / src_div = row of a (null: row of a = row)
 };
+// Activation rows of a tile for `rows` rows in `groups` matrices of n rows: 16
+// (weights streamed), 64 or 256.
+int block_tile_rows(long rows, int groups, int n, int c_dtype, bool swiglu);
+// The product by tiles of g.tile_rows rows.  SwiGLU: tiles of 16 rows write f32
+// [m][n] to c, larger ones E4M3 codes to c and their scales to c_s.
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st);
+hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st);  // mx_block_stream.hip
+hipError_t launch_block_tile(int c_dtype, const BlockGemmArgs& g, hipStream_t st);    // mx_block_tile.hip
 
 }  // namespace mx

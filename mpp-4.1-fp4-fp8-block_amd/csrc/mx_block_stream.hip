@@ -1,0 +1,159 @@
+// mx_block_stream.hip - products of block-scaled FP8 weights with at most 16
+// activation rows a tile: the weights stream from HBM to registers once.
+#include "mx_block.h"
+#include "mx_block_device.h"
+
+namespace mx {
+namespace {
+
+__device__ __align__(16) const uint8_t kZeros[16] = {};
+
+// v with its lanes' halves of 16 exchanged where MASK has the lane's group of
+// four: old elsewhere.
+template <int MASK>
+__device__ __forceinline__ v4i from_other_half(v4i old, v4i v) {
+  v4i r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = __builtin_amdgcn_update_dpp(old[i], v[i], 0x128, 0xf, MASK, false);
+  return r;
+}
+
+template <int NG>
+struct Step {
+  v4i w[NG][2], a[2];
+  float as, ws[2];
+};
+
+// 16 NG weight rows (SwiGLU: half of them gate, half up) x 16 activation rows;
+// 4 waves take every fourth 128-block of K, D blocks ahead.
+template <int DT, bool DUAL, int NG, int D>
+__global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
+  constexpr int ND = DUAL ? 2 : 1, CH = 16 * NG / ND;  // channels of the workgroup
+  __shared__ float part[4][NG][16][17];
+  const int NT = (g.n + CH - 1) / CH;
+  int row0 = blockIdx.x / NT * 16, rows = min(16, g.m - row0), expert = 0;
+  if (g.tiles) {
+    const int rt = blockIdx.x / NT;
+    if (rt >= *g.n_tiles) return;
+    const RowTile t = g.tiles[rt];
+    row0 = t.row0;
+    rows = t.rows;
+    expert = t.expert;
+  }
+  const int n0 = blockIdx.x % NT * CH;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
+  const int K = g.k, KB = (K + kQBlock - 1) / kQBlock;
+  // A load covers 8 whole rows of 128 bytes: lane l has row l % 8 and chunk
+  // 2 (l / 16) + (l / 8) % 2, and gets its own row's other chunk from the lane
+  // half of 16 away.
+  const int wchunk = 2 * kq + (r16 >> 3);
+  const uint8_t* w[NG][2];
+#pragma unroll
+  for (int i = 0; i < NG; i++)
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int n = n0 + (i % (NG / ND)) * 16 + u * 8 + (r16 & 7);
+      w[i][u] = (DUAL && i >= NG / 2 ? g.w1 : g.w0) + expert * g.w_stride + (size_t)min(n, g.n - 1) * K + wchunk * 16;
+    }
+  const int row = row0 + min(r16, rows - 1), ar = g.src ? g.src[row] / g.src_div : row;
+  const uint8_t* a = g.a + (size_t)ar * K + kq * 32;
+  const float* as = g.a_s + ar;
+  const size_t so = expert * g.s_stride + (size_t)(n0 / kQBlock) * KB;
+  const float *s0 = g.s0 + so, *s1 = (DUAL ? g.s1 : g.s0) + so;
+  const uint8_t* zeros = kZeros;
+  asm volatile("" : "+v"(zeros));  // a value, not a constant: selects, where the compiler would branch
+
+  auto load = [&](int kb, Step<NG>& s) {
+    const size_t o = (size_t)kb * kQBlock;
+    const int left = K - kb * kQBlock;  // chunks past K are zero on both sides: what lies there may be NaN
+    const bool win = wchunk * 16 < left;
+#pragma unroll
+    for (int i = 0; i < NG; i++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) s.w[i][u] = *reinterpret_cast<const v4i*>(win ? w[i][u] + o : zeros);
+#pragma unroll
+    for (int u = 0; u < 2; u++) s.a[u] = *reinterpret_cast<const v4i*>(kq * 32 + u * 16 < left ? a + o + u * 16 : zeros);
+    const int kc = min(kb, KB - 1);
+    s.as = as[(size_t)kc * g.a_rows];
+    s.ws[0] = s0[kc];
+    if constexpr (DUAL) s.ws[1] = s1[kc];
+  };
+  v4f acc[NG];
+#pragma unroll
+  for (int i = 0; i < NG; i++) acc[i] = v4f{0, 0, 0, 0};
+  auto use = [&](int kb, const Step<NG>& s) {
+    v8h x[4];
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) x[2 * u + h] = fp8x8_to_f16<BK_E4M3>((uint32_t)s.a[u][2 * h], (uint32_t)s.a[u][2 * h + 1]);
+    float sc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) sc[d] = kb < KB ? s.as * s.ws[d] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NG; i++) {
+      // lanes of the lower half: row r16 of the first load; upper: of the second
+      const v4i c[2] = {from_other_half<0xc>(s.w[i][0], s.w[i][1]), from_other_half<0x3>(s.w[i][1], s.w[i][0])};
+      v4f t = {0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          t = mfma_f16_16x16x32(fp8x8_to_f16<BK_E4M3>((uint32_t)c[u][2 * h], (uint32_t)c[u][2 * h + 1]), x[2 * u + h], t);
+#pragma unroll
+      for (int v = 0; v < 4; v++) acc[i][v] = fmaf(t[v], sc[DUAL && i >= NG / 2 ? 1 : 0], acc[i][v]);
+    }
+  };
+  Step<NG> st[D];
+#pragma unroll
+  for (int d = 0; d < D; d++) load(wave + 4 * d, st[d]);
+  for (int kb = wave; kb < KB; kb += 4 * D) {
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+      use(kb + 4 * d, st[d]);
+      load(kb + 4 * (d + D), st[d]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NG; i++)
+#pragma unroll
+    for (int v = 0; v < 4; v++) part[wave][i][r16][kq * 4 + v] = acc[i][v];
+  __syncthreads();
+  // the waves' sums, in their order
+  for (int o = threadIdx.x; o < 16 * CH; o += 256) {
+    const int r = o / CH, c = o % CH;
+    if (r >= rows || n0 + c >= g.n) continue;
+    float x[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+      const int i = c / 16 + d * (NG / 2);
+      x[d] = ((part[0][i][r][c % 16] + part[1][i][r][c % 16]) + part[2][i][r][c % 16]) + part[3][i][r][c % 16];
+    }
+    float y = x[0];
+    if constexpr (DUAL) y = silu(y) * x[1];
+    store_from_f32<DT>(g.c, (size_t)(row0 + r) * g.n + n0 + c, y);
+  }
+}
+
+template <int DT, bool DUAL, int NG, int D>
+hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
+  constexpr int CH = 16 * NG / (DUAL ? 2 : 1);
+  const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + 15) / 16) * ((g.n + CH - 1) / CH);
+  if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((k_block_stream<DT, DUAL, NG, D>), dim3((unsigned)tiles), dim3(256), 0, st, g);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
+  if (g.w1) return launch_one<MX_DTYPE_F32, true, 2, 4>(g, st);
+  switch (c_dtype) {
+    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 2, 4>(g, st);
+    case MX_DTYPE_F16: return launch_one<MX_DTYPE_F16, false, 2, 4>(g, st);
+    case MX_DTYPE_BF16: return launch_one<MX_DTYPE_BF16, false, 2, 4>(g, st);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace mx

@@ -1,0 +1,303 @@
+// mx_block_tile.hip - tile products of block-scaled FP8 matrices.
+#include <type_traits>
+
+#include "mx_block.h"
+#include "mx_block_device.h"
+#include "mx_convert.h"
+#include "mx_device.h"
+#include "mx_dma.h"
+#include "mx_widen.h"
+
+namespace mx {
+namespace {
+
+constexpr int kPast = 0x7fffff00;  // past every resource's range
+constexpr int lgkm0_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4); }
+__device__ __forceinline__ void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0); }
+__device__ __forceinline__ void dma4(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, lds, 4, 0, 0); }
+
+__device__ __align__(16) const uint8_t kZeros[16] = {};
+
+// TN weight rows (SwiGLU: TN / 2 of gate and the same of up) x TM activation
+// rows, by WN x WM waves, over all of K in stages of one 128-block.
+template <int DT, bool DUAL, int TN, int TM, int WN, int WM, int NS, bool WIDE>
+__global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
+  constexpr int NW = WN * WM, CN = TN / WN, CM = TM / WM, NI = CN / 16, MJ = CM / 16;
+  constexpr int SLOT = (TN + TM) * kQBlock, NDMA = (TN + TM) / 8 / NW, PER = NDMA + 1;
+  constexpr int ND = DUAL ? 2 : 1;  // weight scales of a wave
+  static_assert((TN + TM) / 8 % NW == 0 && TM % 64 == 0, "whole instructions");
+  static_assert(TN / ND <= kQBlock || !DUAL, "one block of mid channels");
+  __shared__ __attribute__((aligned(16))) uint8_t r0[SLOT];
+  __shared__ __attribute__((aligned(16))) uint8_t r1[SLOT];
+  __shared__ __attribute__((aligned(16))) uint8_t r2[NS > 2 ? SLOT : 16];
+  __shared__ __attribute__((aligned(16))) float a0[TM];
+  __shared__ __attribute__((aligned(16))) float a1[TM];
+  __shared__ __attribute__((aligned(16))) float a2[NS > 2 ? TM : 4];
+  __shared__ float wsl[2][kMaxBlocks];
+  __shared__ float amax_l[DUAL ? WN : 1][DUAL ? TM : 1];
+
+  const int NT = (g.n + TN / ND - 1) / (TN / ND);
+  const int total = (g.tiles ? *g.n_tiles : (g.m + TM - 1) / TM) * NT;
+  // an XCD takes a run of neighbouring tiles
+  const int per = (total + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;
+  const int rt = tile / NT, n0 = (tile % NT) * (TN / ND);
+  int row0 = rt * TM, rows = min(TM, g.m - row0), expert = 0;
+  if (g.tiles) {
+    const RowTile t = g.tiles[rt];
+    row0 = t.row0;
+    rows = t.rows;
+    expert = t.expert;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
+  const int K = g.k, KB = (K + kQBlock - 1) / kQBlock;
+
+  // block scales of the weights: the whole of K
+  const size_t so = expert * g.s_stride;
+  for (int i = tid; i < KB; i += 64 * NW) {
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+      // SwiGLU: gate and up; else the tile's two blocks of weight rows
+      const int nb = n0 / kQBlock + (DUAL ? 0 : d);
+      const float* s = (DUAL && d ? g.s1 : g.s0) + so;
+      wsl[d][i] = s[(size_t)min(nb, (g.n - 1) / kQBlock) * KB + i];
+    }
+  }
+
+  // DMA: an instruction moves 8 rows of 128 bytes, 16-byte chunk c of row r to
+  // place c ^ (r % 8), so that the 16 rows of a fragment read cover all banks.
+  // Weights through a buffer resource of the tile's rows (past them: zeros);
+  // activations by address, since a row may lie anywhere.  Chunks past K read as
+  // zero on both sides: what lies there may be NaN.
+  const int tail = (K - (KB - 1) * kQBlock) / 16;  // chunks of the last block
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  constexpr int TW = TN / ND, QW = TN / 8 / NW, QA = NDMA - QW;  // weight rows of a matrix; instructions of a wave
+  static_assert(TN / 8 % NW == 0, "whole instructions");
+  // wave w moves weight rows (q NW + w) 8 ..: with SwiGLU, the first half of q gate
+  const uint32_t wrange = (uint32_t)min(TW, g.n - n0) * (uint32_t)K;
+  const size_t wo = expert * g.w_stride + (size_t)n0 * K;
+  const v4i wrs0 = rsrc_of<true>(g.w0 + wo, wrange), wrs1 = rsrc_of<true>((DUAL ? g.w1 : g.w0) + wo, wrange);
+  const int woff = (wave * 8 + (lane >> 3)) * K + chunk * 16;
+  const uint8_t* src[QA];
+#pragma unroll
+  for (int q = 0; q < QA; q++) {
+    const int row = row0 + min((q * NW + wave) * 8 + (lane >> 3), rows - 1);
+    src[q] = g.a + (size_t)(g.src ? g.src[row] / g.src_div : row) * K + chunk * 16;
+  }
+  const int srow = row0 + min((wave * 64) % TM + lane, rows - 1);
+  const float* ssrc = g.a_s + (g.src ? g.src[srow] / g.src_div : srow);
+  const uint8_t* zeros = kZeros;
+  asm volatile("" : "+v"(zeros));  // a value, not a constant: selects, where the compiler would branch
+  auto slot = [&](auto u) -> uint8_t* {
+    constexpr int U = decltype(u)::value % NS;
+    if constexpr (U == 0) return r0;
+    else if constexpr (U == 1) return r1;
+    else return r2;
+  };
+  auto aslot = [&](auto u) -> float* {
+    constexpr int U = decltype(u)::value % NS;
+    if constexpr (U == 0) return a0;
+    else if constexpr (U == 1) return a1;
+    else return a2;
+  };
+  auto issue = [&](int k, auto u) {
+    uint8_t* s = slot(u);
+    // (no branch: the compiler would move products past it)
+    const bool zero = (k >= KB) | ((k == KB - 1) & (chunk >= tail));
+    const int wk = zero ? kPast : woff + k * kQBlock;
+#pragma unroll
+    for (int q = 0; q < QW; q++) {
+      const bool up = DUAL && q >= QW / 2;
+      llvm_amdgcn_raw_buffer_load_lds_u32(up ? wrs1 : wrs0, (lds_u32)(s + (q * NW + wave) * 1024), 16, wk, (up ? q - QW / 2 : q) * NW * 8 * K, 0, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < QA; q++)
+      dma16(zero ? zeros : src[q] + (size_t)k * kQBlock, s + TN * 128 + (q * NW + wave) * 1024);
+    dma4(ssrc + (size_t)min(k, KB - 1) * g.a_rows, aslot(u) + (wave * 64) % TM);
+  };
+
+  // fragments: lane l has bytes [32 (l / 16), +32) of row l % 16
+  const int sw = r16 & 7, off0 = r16 * 128 + (((2 * kq) ^ sw) << 4), off1 = r16 * 128 + (((2 * kq + 1) ^ sw) << 4);
+  auto wrow = [&](int i) { return DUAL ? (i < NI / 2 ? wn * (CN / 2) + i * 16 : TN / 2 + wn * (CN / 2) + (i - NI / 2) * 16) : wn * CN + i * 16; };
+  auto frag = [&](const uint8_t* s, int row) -> v8i {
+    const v4i lo = *reinterpret_cast<const v4i*>(s + row * 128 + off0), hi = *reinterpret_cast<const v4i*>(s + row * 128 + off1);
+    return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+
+  v4f acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; i++)
+#pragma unroll
+    for (int j = 0; j < MJ; j++) acc[i][j] = v4f{0, 0, 0, 0};
+
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  issue(0, I0{});
+  issue(1, I1{});
+  if constexpr (NS > 2) issue(2, I2{});
+  __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 1) * PER));
+  __builtin_amdgcn_s_barrier();
+  const int wblk = DUAL ? 0 : (wn * CN) / kQBlock;
+
+  // The sums of column j are scaled and added while column j + 1 is multiplied
+  // (t, sc); a stage's weight fragments and its first column's are read at the end
+  // of the stage before.
+  v8i wf[NI], af[2];
+  v8h wh[WIDE ? NI : 1][4];
+  v4f t[2][NI];
+  float sc[2][ND], av[2], ws[ND];
+  auto first = [&](int k, auto u) {
+    const uint8_t* s = slot(u);
+#pragma unroll
+    for (int i = 0; i < NI; i++) wf[i] = frag(s, wrow(i));
+    af[0] = frag(s + TN * 128, wm * CM);
+    av[0] = aslot(u)[wm * CM + r16];
+#pragma unroll
+    for (int d = 0; d < ND; d++) ws[d] = wsl[DUAL ? d : wblk][min(k, KB - 1)];
+  };
+  auto add = [&](int i, int j) {  // column j's sums
+#pragma unroll
+    for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(t[j & 1][i][v], sc[j & 1][DUAL && i >= NI / 2 ? 1 : 0], acc[i][j][v]);
+  };
+#pragma unroll
+  for (int i = 0; i < NI; i++) t[1][i] = v4f{0, 0, 0, 0};
+#pragma unroll
+  for (int d = 0; d < ND; d++) sc[1][d] = 0.0f;
+  static_assert(MJ % 2 == 0, "columns alternate");
+  first(0, I0{});
+
+  auto stage = [&](int k, auto u) {
+    constexpr int U = decltype(u)::value;
+    const uint8_t* s = slot(u);
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) widen4(wf[i], wh[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < MJ; j++) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (j == MJ - 1) {
+        // the stage's fragments are in registers and the next stage has landed
+        __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 2) * PER));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        issue(k + NS, u);
+      } else {
+        af[(j + 1) & 1] = frag(s + TN * 128, wm * CM + (j + 1) * 16);
+        av[(j + 1) & 1] = aslot(u)[wm * CM + (j + 1) * 16 + r16];
+      }
+      v8h xh[4];
+      if constexpr (WIDE) widen4(af[j & 1], xh);
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        if constexpr (WIDE) {
+          t[j & 1][i] = v4f{0, 0, 0, 0};
+#pragma unroll
+          for (int q = 0; q < 4; q++) t[j & 1][i] = mfma_f16_16x16x32(wh[i][q], xh[q], t[j & 1][i]);
+        } else {
+          t[j & 1][i] = mfma_fp8_16x16x128(wf[i], af[j & 1]);
+        }
+        add(i, (j + MJ - 1) % MJ);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; d++) sc[j & 1][d] = av[j & 1] * ws[d];
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    first(k + 1, std::integral_constant<int, U + 1>{});
+  };
+  int k = 0;
+  for (; k + NS <= KB; k += NS) {
+    stage(k, I0{});
+    stage(k + 1, I1{});
+    if constexpr (NS > 2) stage(k + 2, I2{});
+  }
+  if (k < KB) {
+    stage(k, I0{});
+    if constexpr (NS > 2) {
+      if (k + 1 < KB) stage(k + 1, I1{});
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(lgkm0_vm(0));
+#pragma unroll
+  for (int i = 0; i < NI; i++) add(i, MJ - 1);
+
+  if constexpr (DUAL) {
+    // silu(gate) up, then one scale per row and its 128 channels
+#pragma unroll
+    for (int j = 0; j < MJ; j++) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < NI / 2; i++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+          const int c = n0 + wrow(i) + kq * 4 + v;
+          const float x = c < g.n ? silu(acc[i][j][v]) * acc[i + NI / 2][j][v] : 0.0f;
+          acc[i][j][v] = x;
+          amax = max(amax, abs_bits(x));
+        }
+      amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+      amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+      if (kq == 0) amax_l[wn][wm * CM + j * 16 + r16] = __builtin_bit_cast(float, amax);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MJ; j++) {
+      const int r = wm * CM + j * 16 + r16;
+      if (r >= rows) continue;
+      uint32_t amax = 0;
+#pragma unroll
+      for (int w = 0; w < WN; w++) amax = max(amax, __builtin_bit_cast(uint32_t, amax_l[w][r]));
+      const float s = block_scale(amax);
+      if (wn == 0 && kq == 0) g.c_s[(size_t)(n0 / kQBlock) * g.m + row0 + r] = s;
+#pragma unroll
+      for (int i = 0; i < NI / 2; i++) {
+        const int c = n0 + wrow(i) + kq * 4;
+        if (c < g.n) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.c) + (size_t)(row0 + r) * g.n + c) = e4m3x4(acc[i][j], s);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < MJ; j++) {
+      const int r = wm * CM + j * 16 + r16;
+      if (r >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int c = n0 + wrow(i) + kq * 4;
+        store4<DT>(g.c, (size_t)(row0 + r) * g.n + c, acc[i][j], g.n - c, g.n % 4 == 0);
+      }
+    }
+  }
+}
+
+template <int DT, bool DUAL, int TN, int TM, int WN, int WM, int NS, bool WIDE>
+hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
+  const int nt = (g.n + TN / (DUAL ? 2 : 1) - 1) / (TN / (DUAL ? 2 : 1));
+  const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + TM - 1) / TM) * nt;
+  if (tiles > 0x7ffffff0L) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((k_block_tile<DT, DUAL, TN, TM, WN, WM, NS, WIDE>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
+                     st, g);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_block_tile(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
+  const int side = g.tile_rows;
+  if (g.w1) return side == 256 ? launch_one<MX_DTYPE_F32, true, 256, 256, 4, 2, 2, false>(g, st) : launch_one<MX_DTYPE_F32, true, 256, 64, 8, 1, 3, true>(g, st);
+  switch (c_dtype) {
+    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 128, 64, 4, 1, 3, true>(g, st);
+    case MX_DTYPE_F16: return side == 256 ? launch_one<MX_DTYPE_F16, false, 256, 256, 4, 2, 2, false>(g, st) : launch_one<MX_DTYPE_F16, false, 128, 64, 4, 1, 3, true>(g, st);
+    case MX_DTYPE_BF16: return side == 256 ? launch_one<MX_DTYPE_BF16, false, 256, 256, 4, 2, 2, false>(g, st) : launch_one<MX_DTYPE_BF16, false, 128, 64, 4, 1, 3, true>(g, st);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace mx

@@ -7,7 +7,7 @@
 namespace mx {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef float v8f __attribute__((ext_vector_type(8)));
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 
 template <int DT>
 __device__ __forceinline__ float load_as_f32(const void* p, size_t i) {

@@ -141,7 +141,7 @@ int mx_block_quantize(mx_ctx* c, const void* src, int src_dtype, int rows, int k
   if (rows == 0) return MX_OK;
   if (!src || !q || !scales || !is_aligned(src, 16) || !is_aligned(q, 16) || !is_aligned(scales, 4))
     return fail(c, MX_EINVAL, "block quantize buffers must be non-null, source and codes 16-byte and scales 4-byte aligned.");
-  MX_RUN(c, mx::launch_block_quantize(src_dtype, src, rows, k, q, scales, nullptr, mx_ctx_stream(c)));
+  MX_RUN(c, mx::launch_block_quantize(src_dtype, src, rows, k, q, scales, mx_ctx_stream(c)));
   return MX_OK;
 }
 
@@ -150,6 +150,7 @@ int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const ui
   if (!c) return MX_EINVAL;
   if (m < 0 || n <= 0 || k <= 0 || k % 16)
     return fail(c, MX_EINVAL, "block matmul needs m >= 0, n > 0 and k a positive multiple of 16.");
+  if (k > mx::kMaxBlocks * mx::kQBlock) return fail(c, MX_EINVAL, "block matmul k is at most %d.", mx::kMaxBlocks * mx::kQBlock);
   if (!is_float(c_dtype)) return fail(c, MX_EINVAL, "block matmul C must be f32, f16 or bf16.");
   if (m == 0) return MX_OK;
   if (!a || !a_scales || !b || !b_scales || !out || !is_aligned(a, 16) || !is_aligned(b, 16) || !is_aligned(out, 16) ||
@@ -165,6 +166,7 @@ int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const ui
   g.m = m;
   g.n = n;
   g.k = k;
+  g.tile_rows = mx::block_tile_rows(m, 1, n, c_dtype, false);
   MX_RUN(c, mx::launch_block_gemm(c_dtype, g, mx_ctx_stream(c)));
   return MX_OK;
 }
@@ -180,6 +182,8 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   if (int rc = check_experts(c, E)) return rc;
   if (H < 16 || I < 16 || H % 16 || I % 16)
     return fail(c, MX_EINVAL, "Block FP8 needs hidden and intermediate to be positive multiples of 16.");
+  if (H > mx::kMaxBlocks * mx::kQBlock || I > mx::kMaxBlocks * mx::kQBlock)
+    return fail(c, MX_EINVAL, "Block FP8 hidden and intermediate are at most %d.", mx::kMaxBlocks * mx::kQBlock);
   if (dtype != MX_DTYPE_F16 && dtype != MX_DTYPE_BF16) return fail(c, MX_EINVAL, "MoE rows must be f16 or bf16.");
   if (!w) return fail(c, MX_EINVAL, "MLP weight buffers must not be null.");
   const mx_qmatrix* mats[3] = {&w->gate, &w->up, &w->down};
@@ -193,11 +197,17 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   const int n = T * topk;
   size_t off = 0;
   auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
-  const int tile_rows = 64, max_tiles = (n < E ? n : E) + n / tile_rows;
+  // one tile height for both products, so that they share the list of tiles
+  const int used = n < E ? n : E, tile_rows = mx::block_tile_rows(n, used, I, dtype, true), max_tiles = used + n / tile_rows;
+  // Few rows keep the middle and the experts' rows in f32; more of them the
+  // middle in its codes alone and the experts' rows in the rows' type, one
+  // rounding more for half the bytes.
+  const bool few = tile_rows == 16;
+  const int y_dtype = few ? MX_DTYPE_F32 : dtype;
   const size_t o_xq = take((size_t)T * H), o_xs = take((size_t)T * blocks(H) * 4), o_rows = take((size_t)n * 4),
                o_src = take((size_t)n * 4), o_counts = take((size_t)E * 4), o_tiles = take((size_t)max_tiles * sizeof(mx::RowTile)),
-               o_nt = take(4), o_hist = take(mx::dispatch_ws_bytes(n, E)), o_mid = take((size_t)n * I * 4),
-               o_mq = take((size_t)n * I), o_ms = take((size_t)n * blocks(I) * 4), o_y = take((size_t)n * H * 4);
+               o_nt = take(4), o_hist = take(mx::dispatch_ws_bytes(n, E)), o_mid = take(few ? (size_t)n * I * 4 : 0),
+               o_mq = take((size_t)n * I), o_ms = take((size_t)n * blocks(I) * 4), o_y = take((size_t)n * H * size_of(y_dtype));
   void* p = nullptr;
   if (int rc = mx_ctx_workspace(c, off, &p)) return rc;
   uint8_t* ws = static_cast<uint8_t*>(p);
@@ -206,7 +216,7 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
                      reinterpret_cast<int32_t*>(ws + o_src), reinterpret_cast<mx::RowTile*>(ws + o_tiles),
                      reinterpret_cast<int32_t*>(ws + o_nt), tile_rows, reinterpret_cast<int32_t*>(ws + o_hist)};
   MX_RUN(c, mx::launch_dispatch(d, st));
-  MX_RUN(c, mx::launch_block_quantize(dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), nullptr, st));
+  MX_RUN(c, mx::launch_block_quantize(dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), st));
   mx::BlockGemmArgs g{};
   g.a = ws + o_xq;
   g.a_s = reinterpret_cast<float*>(ws + o_xs);
@@ -215,7 +225,8 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   g.w1 = static_cast<const uint8_t*>(w->up.data);
   g.s0 = static_cast<const float*>(w->gate.scales);
   g.s1 = static_cast<const float*>(w->up.scales);
-  g.c = ws + o_mid;
+  g.c = few ? ws + o_mid : ws + o_mq;
+  g.c_s = reinterpret_cast<float*>(ws + o_ms);
   g.m = n;
   g.n = I;
   g.k = H;
@@ -228,7 +239,8 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   g.src = d.src;
   g.src_div = topk;
   MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
-  MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + o_mid, n, I, ws + o_mq, reinterpret_cast<float*>(ws + o_ms), nullptr, st));
+  if (few)
+    MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + o_mid, n, I, ws + o_mq, reinterpret_cast<float*>(ws + o_ms), st));
   g.a = ws + o_mq;
   g.a_s = reinterpret_cast<float*>(ws + o_ms);
   g.a_rows = n;
@@ -239,9 +251,9 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   g.n = H;
   g.k = I;
   g.src = nullptr;
-  MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
+  MX_RUN(c, mx::launch_block_gemm(y_dtype, g, st));
   const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H};
-  MX_RUN(c, mx::launch_combine(MX_DTYPE_F32, dtype, b, st));
+  MX_RUN(c, mx::launch_combine(y_dtype, dtype, b, st));
   return MX_OK;
 }
 

@@ -113,6 +113,27 @@ def test_matmul(dev, m, n, k):
         assert np.all(diff <= R.rounded(ref, err, ct)), (ct, diff.max())
 
 
+@pytest.mark.parametrize("m,n,k", [(700, 16384, 272), (385, 16400, 400), (2050, 4100, 656), (4096, 2048, 128), (257, 32768, 144)])
+@pytest.mark.parametrize("ct", [H, B])
+def test_matmul_on_the_fp8_cores(dev, ct, m, n, k):
+    """Sizes of the 256-row tiles, at random places and in the last rows and columns."""
+    rng = np.random.default_rng(m + n + k)
+    x = (rng.normal(0, 1, (m, k)) * np.exp(rng.normal(0, 1, (m, 1)))).astype(np.float32)
+    q, s = quantize(dev, x, F)
+    rs = R.act_scales(x)
+    wq, ws, wv = weights(dev, rng, 1, n, k)
+    rows = np.unique(np.r_[rng.integers(0, m, 60), 0, m - 1])
+    cols = np.unique(np.r_[rng.integers(0, n, 400), 0, n - 20:n])
+    a = R.act_codes(x, rs) * np.repeat(rs.T, 128, 1)[:, :k].astype(np.float64)
+    ref, err = R.product(a[rows], wv[0][cols], cores=True)
+    c = dev.upload(np.full(m * n + 64, 9, R.np_type(ct)))
+    dev.block_matmul(q, s, wq, ws, c, ct, m, n, k)
+    got = dev.download(c, R.np_type(ct), m * n + 64)
+    assert (got[m * n:] == 9).all()
+    diff = np.abs(R.values_of(got[:m * n].reshape(m, n)[np.ix_(rows, cols)], ct) - ref)
+    assert np.all(diff <= R.rounded(ref, err, ct)), diff.max()
+
+
 @pytest.mark.parametrize("m", [1, 20, 200])
 def test_matmul_repeats_bit_for_bit(dev, m):
     rng = np.random.default_rng(m)
@@ -179,7 +200,7 @@ def expert_case(dev, t, h, i, e, k, dtype, seed, drop=0.0, one=None):
     return x, ids, w, ws, R.bits_of(rng.normal(0, 1, (t, h)), dtype)
 
 
-def expert_ref(x, ids, w, ws, add, dtype):
+def expert_ref(x, ids, w, ws, add, dtype, cores=False):
     """Sum and bound; a slot's row may be rounded once to the rows' type."""
     xv = dequant(x, dtype)
     ref = np.zeros(x.shape) if add is None else R.values_of(add, dtype)
@@ -188,7 +209,7 @@ def expert_ref(x, ids, w, ws, add, dtype):
     for e in range(len(ws[0][2])):
         t, s = np.nonzero(ids == e)
         if t.size:
-            y, ey = R.mlp(xv[t], *[v[2][e] for v in ws])
+            y, ey = R.mlp(xv[t], *[v[2][e] for v in ws], cores=cores)
             ey = R.rounded(y, ey, dtype)
             wt = w[t, s].astype(np.float64)[:, None]
             np.add.at(ref, t, wt * y)
@@ -215,6 +236,28 @@ def test_experts(dev, dtype, t, h, i, e, k, add):
     ref, err = expert_ref(x, ids, w, ws, base if add else None, dtype)
     got = run_experts(dev, x, ids, w, ws, base if add else None, dtype)
     assert np.all(np.abs(got - ref) <= err)
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("t,h,i,e,k", [(1100, 256, 2064, 4, 1), (1000, 400, 1040, 8, 2)])
+def test_experts_on_the_fp8_cores(dev, dtype, t, h, i, e, k):
+    x, ids, w, ws, base = expert_case(dev, t, h, i, e, k, dtype, t + h, drop=0.05)
+    ref, err = expert_ref(x, ids, w, ws, base, dtype, cores=True)
+    got = run_experts(dev, x, ids, w, ws, base, dtype)
+    assert np.all(np.abs(got - ref) <= err)
+
+
+def test_format_mlp_on_the_fp8_cores(dev):
+    t, h, i = 600, 272, 8208
+    rng = np.random.default_rng(t)
+    x = R.bits_of(rng.normal(0, 1, (t, h)), H)
+    ws = [weights(dev, rng, 1, n, k, std=0.05) for n, k in ((i, h), (i, h), (h, i))]
+    out = dev.alloc(t * h * 2)
+    dev.fmt_mlp_forward(M.WFMT_FP8_BLOCK, t, h, i, dev.upload(x), M.Device.weights(*[w[:2] for w in ws]), out)
+    rows = np.unique(np.r_[rng.integers(0, t, 40), 0, t - 1])
+    y, err = R.mlp(dequant(x, H)[rows], *[w[2][0] for w in ws], cores=True)
+    got = R.values_of(dev.download(out, np.float16, (t, h)), H)[rows]
+    assert np.all(np.abs(got - y) <= R.rounded(y, err, H))
 
 
 @pytest.mark.parametrize("t", [1, 40, 300])
