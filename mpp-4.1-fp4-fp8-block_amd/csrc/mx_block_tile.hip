@@ -13,10 +13,18 @@ namespace {
 
 constexpr int kPast = 0x7fffff00;  // past every resource's range
 constexpr int lgkm0_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4); }
-__device__ __forceinline__ void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0); }
+__device__ __forceinline__ void dma16(v4i rsrc, void* lds, int lane_offset, int offset) {
+  llvm_amdgcn_raw_buffer_load_lds_u32(rsrc, (lds_u32)lds, 16, lane_offset, offset, 0, 0);
+}
 __device__ __forceinline__ void dma4(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, lds, 4, 0, 0); }
 
-__device__ __align__(16) const uint8_t kZeros[16] = {};
+// The 64 banks hold two rows of 128 bytes.  A 16-byte read takes its lanes in
+// groups of 16: lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31, and the same 32
+// on.  Lane l reads chunk 2 (l / 16) + h of row l % 16, so a group has every row
+// once, rows 4 to 11 with a chunk 2 further (or nearer) than the others; with
+// this key its reads go to 16 places that are all different (the counter of bank
+// conflicts went from 4 a read to 0).
+__device__ __forceinline__ int place_key(int r) { return (r >> 1 & 1) | (r >> 3 & 1) * 6; }
 
 // TN weight rows (SwiGLU: TN / 2 of gate and the same of up) x TM activation
 // rows, by WN x WM waves, over all of K in stages of one 128-block.
@@ -36,12 +44,13 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   __shared__ float wsl[2][kMaxBlocks];
   __shared__ float amax_l[DUAL ? WN : 1][DUAL ? TM : 1];
 
-  const int NT = (g.n + TN / ND - 1) / (TN / ND);
-  const int total = (g.tiles ? *g.n_tiles : (g.m + TM - 1) / TM) * NT;
-  // an XCD takes a run of neighbouring tiles
-  const int per = (total + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const int NT = (g.n + TN / ND - 1) / (TN / ND), MT = g.tiles ? *g.n_tiles : (g.m + TM - 1) / TM;
+  // An XCD takes a run of neighbouring tiles, 8 weight tiles by all row tiles: its
+  // 32 CUs then work on about 8 weight and 4 row tiles and fetch each once.
+  const int total = MT * NT, per = (total + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;
-  const int rt = tile / NT, n0 = (tile % NT) * (TN / ND);
+  const int grp = tile / (8 * MT), in = tile % (8 * MT), gw = min(8, NT - grp * 8);
+  const int rt = in / gw, n0 = (grp * 8 + in % gw) * (TN / ND);
   int row0 = rt * TM, rows = min(TM, g.m - row0), expert = 0;
   if (g.tiles) {
     const RowTile t = g.tiles[rt];
@@ -66,12 +75,13 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   }
 
   // DMA: an instruction moves 8 rows of 128 bytes, 16-byte chunk c of row r to
-  // place c ^ (r % 8), so that the 16 rows of a fragment read cover all banks.
-  // Weights through a buffer resource of the tile's rows (past them: zeros);
-  // activations by address, since a row may lie anywhere.  Chunks past K read as
-  // zero on both sides: what lies there may be NaN.
+  // place c ^ place_key(r).
+  // Through buffer resources of the tile's rows (of a whole batch whose rows are
+  // picked): what lies past them reads as zero.  So do chunks past K, on both
+  // sides: what lies there may be NaN.
   const int tail = (K - (KB - 1) * kQBlock) / 16;  // chunks of the last block
-  const int chunk = (lane & 7) ^ (lane >> 3);
+  const int chunk = (lane & 7) ^ place_key((wave & 1) * 8 + (lane >> 3));
+  static_assert(NW % 2 == 0, "a wave's groups of 8 rows are all even or all odd");
   constexpr int TW = TN / ND, QW = TN / 8 / NW, QA = NDMA - QW;  // weight rows of a matrix; instructions of a wave
   static_assert(TN / 8 % NW == 0, "whole instructions");
   // wave w moves weight rows (q NW + w) 8 ..: with SwiGLU, the first half of q gate
@@ -79,16 +89,15 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   const size_t wo = expert * g.w_stride + (size_t)n0 * K;
   const v4i wrs0 = rsrc_of<true>(g.w0 + wo, wrange), wrs1 = rsrc_of<true>((DUAL ? g.w1 : g.w0) + wo, wrange);
   const int woff = (wave * 8 + (lane >> 3)) * K + chunk * 16;
-  const uint8_t* src[QA];
+  const v4i ars = rsrc_of<true>(g.src ? g.a : g.a + (size_t)row0 * K, (uint32_t)(g.src ? g.a_rows : rows) * (uint32_t)K);
+  int aoff[QA];
 #pragma unroll
   for (int q = 0; q < QA; q++) {
-    const int row = row0 + min((q * NW + wave) * 8 + (lane >> 3), rows - 1);
-    src[q] = g.a + (size_t)(g.src ? g.src[row] / g.src_div : row) * K + chunk * 16;
+    const int r = min((q * NW + wave) * 8 + (lane >> 3), rows - 1);
+    aoff[q] = (g.src ? g.src[row0 + r] / g.src_div : r) * K + chunk * 16;
   }
   const int srow = row0 + min((wave * 64) % TM + lane, rows - 1);
   const float* ssrc = g.a_s + (g.src ? g.src[srow] / g.src_div : srow);
-  const uint8_t* zeros = kZeros;
-  asm volatile("" : "+v"(zeros));  // a value, not a constant: selects, where the compiler would branch
   auto slot = [&](auto u) -> uint8_t* {
     constexpr int U = decltype(u)::value % NS;
     if constexpr (U == 0) return r0;
@@ -101,24 +110,30 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
     else if constexpr (U == 1) return a1;
     else return a2;
   };
-  auto issue = [&](int k, auto u) {
+  // A stage's loads in four parts, so that no wave waits long to issue them.
+  constexpr int PARTS = 4;
+  auto issue = [&](int k, auto u, int p) {
     uint8_t* s = slot(u);
     // (no branch: the compiler would move products past it)
     const bool zero = (k >= KB) | ((k == KB - 1) & (chunk >= tail));
-    const int wk = zero ? kPast : woff + k * kQBlock;
+    const int ko = k * kQBlock;
 #pragma unroll
-    for (int q = 0; q < QW; q++) {
+    for (int q = p * QW / PARTS; q < (p + 1) * QW / PARTS; q++) {
       const bool up = DUAL && q >= QW / 2;
-      llvm_amdgcn_raw_buffer_load_lds_u32(up ? wrs1 : wrs0, (lds_u32)(s + (q * NW + wave) * 1024), 16, wk, (up ? q - QW / 2 : q) * NW * 8 * K, 0, 0);
+      dma16(up ? wrs1 : wrs0, s + (q * NW + wave) * 1024, zero ? kPast : woff, ko + (up ? q - QW / 2 : q) * NW * 8 * K);
     }
 #pragma unroll
-    for (int q = 0; q < QA; q++)
-      dma16(zero ? zeros : src[q] + (size_t)k * kQBlock, s + TN * 128 + (q * NW + wave) * 1024);
-    dma4(ssrc + (size_t)min(k, KB - 1) * g.a_rows, aslot(u) + (wave * 64) % TM);
+    for (int q = p * QA / PARTS; q < (p + 1) * QA / PARTS; q++)
+      dma16(ars, s + TN * 128 + (q * NW + wave) * 1024, zero ? kPast : aoff[q], ko);
+    if (p == PARTS - 1) dma4(ssrc + (size_t)min(k, KB - 1) * g.a_rows, aslot(u) + (wave * 64) % TM);
+  };
+  auto issue_all = [&](int k, auto u) {
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) issue(k, u, p);
   };
 
   // fragments: lane l has bytes [32 (l / 16), +32) of row l % 16
-  const int sw = r16 & 7, off0 = r16 * 128 + (((2 * kq) ^ sw) << 4), off1 = r16 * 128 + (((2 * kq + 1) ^ sw) << 4);
+  const int sw = place_key(r16), off0 = r16 * 128 + (((2 * kq) ^ sw) << 4), off1 = r16 * 128 + (((2 * kq + 1) ^ sw) << 4);
   auto wrow = [&](int i) { return DUAL ? (i < NI / 2 ? wn * (CN / 2) + i * 16 : TN / 2 + wn * (CN / 2) + (i - NI / 2) * 16) : wn * CN + i * 16; };
   auto frag = [&](const uint8_t* s, int row) -> v8i {
     const v4i lo = *reinterpret_cast<const v4i*>(s + row * 128 + off0), hi = *reinterpret_cast<const v4i*>(s + row * 128 + off1);
@@ -134,43 +149,50 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
-  issue(0, I0{});
-  issue(1, I1{});
-  if constexpr (NS > 2) issue(2, I2{});
-  __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 1) * PER));
+  issue_all(0, I0{});
+  if constexpr (NS > 2) issue_all(1, I1{});
+  issue(NS - 1, std::integral_constant<int, NS - 1>{}, 0);
+  __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 2) * PER + QW / PARTS + QA / PARTS));
   __builtin_amdgcn_s_barrier();
   const int wblk = DUAL ? 0 : (wn * CN) / kQBlock;
 
   // The sums of column j are scaled and added while column j + 1 is multiplied
-  // (t, sc); a stage's weight fragments and its first column's are read at the end
-  // of the stage before.
+  // (t, sc).  Over the products of a stage's last column, past the barrier that
+  // ends its reads, go the next stage's first column and weight fragments (each
+  // after the last use of its registers) and the first loads into the slot; the
+  // other loads over the stage's first columns.  (Columns two ahead measured the
+  // same where they fit the registers, and spill here.)
   v8i wf[NI], af[2];
   v8h wh[WIDE ? NI : 1][4];
-  v4f t[2][NI];
+  v4f t[NI];
   float sc[2][ND], av[2], ws[ND];
-  auto first = [&](int k, auto u) {
-    const uint8_t* s = slot(u);
-#pragma unroll
-    for (int i = 0; i < NI; i++) wf[i] = frag(s, wrow(i));
-    af[0] = frag(s + TN * 128, wm * CM);
-    av[0] = aslot(u)[wm * CM + r16];
+  auto column = [&](auto u, int j) {
+    af[j & 1] = frag(slot(u) + TN * 128, wm * CM + j * 16);
+    av[j & 1] = aslot(u)[wm * CM + j * 16 + r16];
+  };
+  auto weights = [&](auto u, int i) { wf[i] = frag(slot(u), wrow(i)); };
+  auto block_scales = [&](int k) {
 #pragma unroll
     for (int d = 0; d < ND; d++) ws[d] = wsl[DUAL ? d : wblk][min(k, KB - 1)];
   };
   auto add = [&](int i, int j) {  // column j's sums
 #pragma unroll
-    for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(t[j & 1][i][v], sc[j & 1][DUAL && i >= NI / 2 ? 1 : 0], acc[i][j][v]);
+    for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(t[i][v], sc[j & 1][DUAL && i >= NI / 2 ? 1 : 0], acc[i][j][v]);
   };
 #pragma unroll
-  for (int i = 0; i < NI; i++) t[1][i] = v4f{0, 0, 0, 0};
+  for (int i = 0; i < NI; i++) t[i] = v4f{0, 0, 0, 0};
 #pragma unroll
   for (int d = 0; d < ND; d++) sc[1][d] = 0.0f;
-  static_assert(MJ % 2 == 0, "columns alternate");
-  first(0, I0{});
+  static_assert(MJ % 2 == 0 && MJ >= PARTS, "columns alternate, and hold a stage's parts");
+  column(I0{}, 0);
+  block_scales(0);
+#pragma unroll
+  for (int i = 0; i < NI; i++) weights(I0{}, i);
 
   auto stage = [&](int k, auto u) {
     constexpr int U = decltype(u)::value;
-    const uint8_t* s = slot(u);
+    using Next = std::integral_constant<int, (U + 1) % NS>;
+    using Last = std::integral_constant<int, (U + NS - 1) % NS>;
     if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < NI; i++) widen4(wf[i], wh[i]);
@@ -178,40 +200,44 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
 #pragma unroll
     for (int j = 0; j < MJ; j++) {
       __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < ND; d++) sc[j & 1][d] = av[j & 1] * ws[d];
       if (j == MJ - 1) {
         // the stage's fragments are in registers and the next stage has landed
         __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 2) * PER));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        issue(k + NS, u);
+        column(Next{}, 0);
+        block_scales(k + 1);
+        issue(k + NS, u, 0);
       } else {
-        af[(j + 1) & 1] = frag(s + TN * 128, wm * CM + (j + 1) * 16);
-        av[(j + 1) & 1] = aslot(u)[wm * CM + (j + 1) * 16 + r16];
+        column(u, j + 1);
+        if (j + 1 < PARTS) issue(k + NS - 1, Last{}, j + 1);
       }
       v8h xh[4];
       if constexpr (WIDE) widen4(af[j & 1], xh);
 #pragma unroll
       for (int i = 0; i < NI; i++) {
-        if constexpr (WIDE) {
-          t[j & 1][i] = v4f{0, 0, 0, 0};
-#pragma unroll
-          for (int q = 0; q < 4; q++) t[j & 1][i] = mfma_f16_16x16x32(wh[i][q], xh[q], t[j & 1][i]);
-        } else {
-          t[j & 1][i] = mfma_fp8_16x16x128(wf[i], af[j & 1]);
-        }
         add(i, (j + MJ - 1) % MJ);
+        if constexpr (WIDE) {
+          t[i] = v4f{0, 0, 0, 0};
+#pragma unroll
+          for (int q = 0; q < 4; q++) t[i] = mfma_f16_16x16x32(wh[i][q], xh[q], t[i]);
+        } else {
+          t[i] = mfma_fp8_16x16x128(wf[i], af[j & 1]);
+        }
+        if (j == MJ - 1) weights(Next{}, i);
       }
 #pragma unroll
-      for (int d = 0; d < ND; d++) sc[j & 1][d] = av[j & 1] * ws[d];
-#pragma unroll
       for (int i = 0; i < NI; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0);
+        if (j == MJ - 1) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    first(k + 1, std::integral_constant<int, U + 1>{});
   };
   int k = 0;
   for (; k + NS <= KB; k += NS) {

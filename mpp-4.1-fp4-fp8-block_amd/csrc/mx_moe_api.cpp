@@ -48,6 +48,72 @@ int check_experts(mx_ctx* c, int experts) {
   return MX_OK;
 }
 
+// One pass of mx_moe_block_forward over T >= 1 tokens.
+int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x, int dtype, const int32_t* ids,
+                  const float* weights, const mx_mlp_weights* w, const void* add, void* out) {
+  const int n = T * topk;
+  size_t off = 0;
+  auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
+  // one tile height for both products, so that they share the list of tiles
+  const int used = n < E ? n : E, tile_rows = mx::block_tile_rows(n, used, I, dtype, true), max_tiles = used + n / tile_rows;
+  // Few rows keep the middle and the experts' rows in f32; more of them the
+  // middle in its codes alone and the experts' rows in the rows' type, one
+  // rounding more for half the bytes.
+  const bool few = tile_rows == 16;
+  const int y_dtype = few ? MX_DTYPE_F32 : dtype;
+  const size_t o_xq = take((size_t)T * H), o_xs = take((size_t)T * blocks(H) * 4), o_rows = take((size_t)n * 4),
+               o_src = take((size_t)n * 4), o_counts = take((size_t)E * 4), o_tiles = take((size_t)max_tiles * sizeof(mx::RowTile)),
+               o_nt = take(4), o_hist = take(mx::dispatch_ws_bytes(n, E)), o_mid = take(few ? (size_t)n * I * 4 : 0),
+               o_mq = take((size_t)n * I), o_ms = take((size_t)n * blocks(I) * 4), o_y = take((size_t)n * H * size_of(y_dtype));
+  void* p = nullptr;
+  if (int rc = mx_ctx_workspace(c, off, &p)) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(p);
+  hipStream_t st = mx_ctx_stream(c);
+  mx::DispatchArgs d{ids, n, E, reinterpret_cast<int32_t*>(ws + o_counts), reinterpret_cast<int32_t*>(ws + o_rows),
+                     reinterpret_cast<int32_t*>(ws + o_src), reinterpret_cast<mx::RowTile*>(ws + o_tiles),
+                     reinterpret_cast<int32_t*>(ws + o_nt), tile_rows, reinterpret_cast<int32_t*>(ws + o_hist)};
+  MX_RUN(c, mx::launch_dispatch(d, st));
+  MX_RUN(c, mx::launch_block_quantize(dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), st));
+  mx::BlockGemmArgs g{};
+  g.a = ws + o_xq;
+  g.a_s = reinterpret_cast<float*>(ws + o_xs);
+  g.a_rows = T;
+  g.w0 = static_cast<const uint8_t*>(w->gate.data);
+  g.w1 = static_cast<const uint8_t*>(w->up.data);
+  g.s0 = static_cast<const float*>(w->gate.scales);
+  g.s1 = static_cast<const float*>(w->up.scales);
+  g.c = few ? ws + o_mid : ws + o_mq;
+  g.c_s = reinterpret_cast<float*>(ws + o_ms);
+  g.m = n;
+  g.n = I;
+  g.k = H;
+  g.tiles = d.tiles;
+  g.n_tiles = d.n_tiles;
+  g.max_tiles = max_tiles;
+  g.tile_rows = tile_rows;
+  g.w_stride = (size_t)I * H;
+  g.s_stride = (size_t)blocks(I) * blocks(H);
+  g.src = d.src;
+  g.src_div = topk;
+  MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
+  if (few)
+    MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + o_mid, n, I, ws + o_mq, reinterpret_cast<float*>(ws + o_ms), st));
+  g.a = ws + o_mq;
+  g.a_s = reinterpret_cast<float*>(ws + o_ms);
+  g.a_rows = n;
+  g.w0 = static_cast<const uint8_t*>(w->down.data);
+  g.w1 = nullptr;
+  g.s0 = static_cast<const float*>(w->down.scales);
+  g.c = ws + o_y;
+  g.n = H;
+  g.k = I;
+  g.src = nullptr;
+  MX_RUN(c, mx::launch_block_gemm(y_dtype, g, st));
+  const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H};
+  MX_RUN(c, mx::launch_combine(y_dtype, dtype, b, st));
+  return MX_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -194,66 +260,15 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   if (!x || !ids || !weights || !out) return fail(c, MX_EINVAL, "MoE buffers must not be null.");
   if (!is_aligned(x, 16) || !is_aligned(out, 16) || !is_aligned(add, 16) || !is_aligned(ids, 4) || !is_aligned(weights, 4))
     return fail(c, MX_EINVAL, "MoE rows must be 16-byte aligned, ids and weights 4-byte.");
-  const int n = T * topk;
-  size_t off = 0;
-  auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
-  // one tile height for both products, so that they share the list of tiles
-  const int used = n < E ? n : E, tile_rows = mx::block_tile_rows(n, used, I, dtype, true), max_tiles = used + n / tile_rows;
-  // Few rows keep the middle and the experts' rows in f32; more of them the
-  // middle in its codes alone and the experts' rows in the rows' type, one
-  // rounding more for half the bytes.
-  const bool few = tile_rows == 16;
-  const int y_dtype = few ? MX_DTYPE_F32 : dtype;
-  const size_t o_xq = take((size_t)T * H), o_xs = take((size_t)T * blocks(H) * 4), o_rows = take((size_t)n * 4),
-               o_src = take((size_t)n * 4), o_counts = take((size_t)E * 4), o_tiles = take((size_t)max_tiles * sizeof(mx::RowTile)),
-               o_nt = take(4), o_hist = take(mx::dispatch_ws_bytes(n, E)), o_mid = take(few ? (size_t)n * I * 4 : 0),
-               o_mq = take((size_t)n * I), o_ms = take((size_t)n * blocks(I) * 4), o_y = take((size_t)n * H * size_of(y_dtype));
-  void* p = nullptr;
-  if (int rc = mx_ctx_workspace(c, off, &p)) return rc;
-  uint8_t* ws = static_cast<uint8_t*>(p);
-  hipStream_t st = mx_ctx_stream(c);
-  mx::DispatchArgs d{ids, n, E, reinterpret_cast<int32_t*>(ws + o_counts), reinterpret_cast<int32_t*>(ws + o_rows),
-                     reinterpret_cast<int32_t*>(ws + o_src), reinterpret_cast<mx::RowTile*>(ws + o_tiles),
-                     reinterpret_cast<int32_t*>(ws + o_nt), tile_rows, reinterpret_cast<int32_t*>(ws + o_hist)};
-  MX_RUN(c, mx::launch_dispatch(d, st));
-  MX_RUN(c, mx::launch_block_quantize(dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), st));
-  mx::BlockGemmArgs g{};
-  g.a = ws + o_xq;
-  g.a_s = reinterpret_cast<float*>(ws + o_xs);
-  g.a_rows = T;
-  g.w0 = static_cast<const uint8_t*>(w->gate.data);
-  g.w1 = static_cast<const uint8_t*>(w->up.data);
-  g.s0 = static_cast<const float*>(w->gate.scales);
-  g.s1 = static_cast<const float*>(w->up.scales);
-  g.c = few ? ws + o_mid : ws + o_mq;
-  g.c_s = reinterpret_cast<float*>(ws + o_ms);
-  g.m = n;
-  g.n = I;
-  g.k = H;
-  g.tiles = d.tiles;
-  g.n_tiles = d.n_tiles;
-  g.max_tiles = max_tiles;
-  g.tile_rows = tile_rows;
-  g.w_stride = (size_t)I * H;
-  g.s_stride = (size_t)blocks(I) * blocks(H);
-  g.src = d.src;
-  g.src_div = topk;
-  MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
-  if (few)
-    MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + o_mid, n, I, ws + o_mq, reinterpret_cast<float*>(ws + o_ms), st));
-  g.a = ws + o_mq;
-  g.a_s = reinterpret_cast<float*>(ws + o_ms);
-  g.a_rows = n;
-  g.w0 = static_cast<const uint8_t*>(w->down.data);
-  g.w1 = nullptr;
-  g.s0 = static_cast<const float*>(w->down.scales);
-  g.c = ws + o_y;
-  g.n = H;
-  g.k = I;
-  g.src = nullptr;
-  MX_RUN(c, mx::launch_block_gemm(y_dtype, g, st));
-  const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H};
-  MX_RUN(c, mx::launch_combine(y_dtype, dtype, b, st));
+  // The picked rows of x are addressed by 31 bits: larger batches in parts.
+  const int most = (int)(0x7fff0000u / (uint32_t)H);
+  for (int t = 0; t < T; t += most) {
+    const size_t row = (size_t)t * H * 2;
+    const int rc = block_experts(c, T - t < most ? T - t : most, H, I, E, topk, static_cast<const uint8_t*>(x) + row, dtype,
+                                 ids + (size_t)t * topk, weights + (size_t)t * topk, w,
+                                 add ? static_cast<const uint8_t*>(add) + row : nullptr, static_cast<uint8_t*>(out) + row);
+    if (rc) return rc;
+  }
   return MX_OK;
 }
 
