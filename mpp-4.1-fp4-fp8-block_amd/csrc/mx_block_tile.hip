@@ -58,7 +58,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
     rows = t.rows;
     expert = t.expert;
   }
-  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, kq = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
   const int K = g.k, KB = (K + kQBlock - 1) / kQBlock;
 
@@ -93,8 +93,8 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   int aoff[QA];
 #pragma unroll
   for (int q = 0; q < QA; q++) {
-    const int r = min((q * NW + wave) * 8 + (lane >> 3), rows - 1);
-    aoff[q] = (g.src ? g.src[row0 + r] / g.src_div : r) * K + chunk * 16;
+    const int r = (q * NW + wave) * 8 + (lane >> 3), ra = min(r, rows - 1);
+    aoff[q] = r < rows ? (g.src ? g.src[row0 + ra] / g.src_div : ra) * K + chunk * 16 : kPast;
   }
   const int srow = row0 + min((wave * 64) % TM + lane, rows - 1);
   const float* ssrc = g.a_s + (g.src ? g.src[srow] / g.src_div : srow);
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   };
   // A stage's loads in four parts, so that no wave waits long to issue them.
   constexpr int PARTS = 4;
-  auto issue = [&](int k, auto u, int p) {
+  auto issue = [&](int k, auto u, int p) __attribute__((always_inline)) {
     uint8_t* s = slot(u);
     // (no branch: the compiler would move products past it)
     const bool zero = (k >= KB) | ((k == KB - 1) & (chunk >= tail));
@@ -132,20 +132,6 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
     for (int p = 0; p < PARTS; p++) issue(k, u, p);
   };
 
-  // fragments: lane l has bytes [32 (l / 16), +32) of row l % 16
-  const int sw = place_key(r16), off0 = r16 * 128 + (((2 * kq) ^ sw) << 4), off1 = r16 * 128 + (((2 * kq + 1) ^ sw) << 4);
-  auto wrow = [&](int i) { return DUAL ? (i < NI / 2 ? wn * (CN / 2) + i * 16 : TN / 2 + wn * (CN / 2) + (i - NI / 2) * 16) : wn * CN + i * 16; };
-  auto frag = [&](const uint8_t* s, int row) -> v8i {
-    const v4i lo = *reinterpret_cast<const v4i*>(s + row * 128 + off0), hi = *reinterpret_cast<const v4i*>(s + row * 128 + off1);
-    return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
-
-  v4f acc[NI][MJ];
-#pragma unroll
-  for (int i = 0; i < NI; i++)
-#pragma unroll
-    for (int j = 0; j < MJ; j++) acc[i][j] = v4f{0, 0, 0, 0};
-
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
@@ -155,6 +141,32 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 2) * PER + QW / PARTS + QA / PARTS));
   __builtin_amdgcn_s_barrier();
   const int wblk = DUAL ? 0 : (wn * CN) / kQBlock;
+
+  // The rest with as many columns as have rows (the waves' registers are those of
+  // the whole tile).
+  auto body = [&](auto columns) __attribute__((always_inline)) {
+  constexpr int MC = decltype(columns)::value;
+  static_assert(MC % 2 == 0 && MC >= PARTS, "columns alternate, and hold a stage's parts");
+  // fragments: lane l has bytes [32 (l / 16), +32) of row l % 16.  Wave wm takes
+  // every WM-th run of 16 activation rows, so that the waves of a tile with few
+  // rows are left with equally many.
+  auto arow = [&](int j) { return (j * WM + wm) * 16; };
+  int mine = lane;
+  asm volatile("" : "+v"(mine));  // (a value of this body: the bodies' common parts are not worked out before them)
+  const int r16 = mine & 15, kq = mine >> 4;
+  const int sw = place_key(r16), off0 = r16 * 128 + (((2 * kq) ^ sw) << 4), off1 = r16 * 128 + (((2 * kq + 1) ^ sw) << 4);
+  auto wrow = [&](int i) { return DUAL ? (i < NI / 2 ? wn * (CN / 2) + i * 16 : TN / 2 + wn * (CN / 2) + (i - NI / 2) * 16) : wn * CN + i * 16; };
+  auto frag = [&](const uint8_t* s, int row) __attribute__((always_inline)) -> v8i {
+    const v4i lo = *reinterpret_cast<const v4i*>(s + row * 128 + off0), hi = *reinterpret_cast<const v4i*>(s + row * 128 + off1);
+    return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+
+  v4f acc[NI][MC];
+#pragma unroll
+  for (int i = 0; i < NI; i++)
+#pragma unroll
+    for (int j = 0; j < MC; j++) acc[i][j] = v4f{0, 0, 0, 0};
+
 
   // The sums of column j are scaled and added while column j + 1 is multiplied
   // (t, sc).  Over the products of a stage's last column, past the barrier that
@@ -166,16 +178,16 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   v8h wh[WIDE ? NI : 1][4];
   v4f t[NI];
   float sc[2][ND], av[2], ws[ND];
-  auto column = [&](auto u, int j) {
-    af[j & 1] = frag(slot(u) + TN * 128, wm * CM + j * 16);
-    av[j & 1] = aslot(u)[wm * CM + j * 16 + r16];
+  auto column = [&](auto u, int j) __attribute__((always_inline)) {
+    af[j & 1] = frag(slot(u) + TN * 128, arow(j));
+    av[j & 1] = aslot(u)[arow(j) + r16];
   };
-  auto weights = [&](auto u, int i) { wf[i] = frag(slot(u), wrow(i)); };
+  auto weights = [&](auto u, int i) __attribute__((always_inline)) { wf[i] = frag(slot(u), wrow(i)); };
   auto block_scales = [&](int k) {
 #pragma unroll
     for (int d = 0; d < ND; d++) ws[d] = wsl[DUAL ? d : wblk][min(k, KB - 1)];
   };
-  auto add = [&](int i, int j) {  // column j's sums
+  auto add = [&](int i, int j) __attribute__((always_inline)) {  // column j's sums
 #pragma unroll
     for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(t[i][v], sc[j & 1][DUAL && i >= NI / 2 ? 1 : 0], acc[i][j][v]);
   };
@@ -183,13 +195,12 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   for (int i = 0; i < NI; i++) t[i] = v4f{0, 0, 0, 0};
 #pragma unroll
   for (int d = 0; d < ND; d++) sc[1][d] = 0.0f;
-  static_assert(MJ % 2 == 0 && MJ >= PARTS, "columns alternate, and hold a stage's parts");
   column(I0{}, 0);
   block_scales(0);
 #pragma unroll
   for (int i = 0; i < NI; i++) weights(I0{}, i);
 
-  auto stage = [&](int k, auto u) {
+  auto stage = [&](int k, auto u) __attribute__((always_inline)) {
     constexpr int U = decltype(u)::value;
     using Next = std::integral_constant<int, (U + 1) % NS>;
     using Last = std::integral_constant<int, (U + NS - 1) % NS>;
@@ -198,11 +209,11 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
       for (int i = 0; i < NI; i++) widen4(wf[i], wh[i]);
     }
 #pragma unroll
-    for (int j = 0; j < MJ; j++) {
+    for (int j = 0; j < MC; j++) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int d = 0; d < ND; d++) sc[j & 1][d] = av[j & 1] * ws[d];
-      if (j == MJ - 1) {
+      if (j == MC - 1) {
         // the stage's fragments are in registers and the next stage has landed
         __builtin_amdgcn_s_waitcnt(lgkm0_vm((NS - 2) * PER));
         __builtin_amdgcn_s_barrier();
@@ -218,7 +229,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
       if constexpr (WIDE) widen4(af[j & 1], xh);
 #pragma unroll
       for (int i = 0; i < NI; i++) {
-        add(i, (j + MJ - 1) % MJ);
+        add(i, (j + MC - 1) % MC);
         if constexpr (WIDE) {
           t[i] = v4f{0, 0, 0, 0};
 #pragma unroll
@@ -226,13 +237,13 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
         } else {
           t[i] = mfma_fp8_16x16x128(wf[i], af[j & 1]);
         }
-        if (j == MJ - 1) weights(Next{}, i);
+        if (j == MC - 1) weights(Next{}, i);
       }
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
         __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0);
-        if (j == MJ - 1) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+        if (j == MC - 1) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
         else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
       }
@@ -253,12 +264,11 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   }
   __builtin_amdgcn_s_waitcnt(lgkm0_vm(0));
 #pragma unroll
-  for (int i = 0; i < NI; i++) add(i, MJ - 1);
-
+  for (int i = 0; i < NI; i++) add(i, MC - 1);
   if constexpr (DUAL) {
     // silu(gate) up, then one scale per row and its 128 channels
 #pragma unroll
-    for (int j = 0; j < MJ; j++) {
+    for (int j = 0; j < MC; j++) {
       uint32_t amax = 0;
 #pragma unroll
       for (int i = 0; i < NI / 2; i++)
@@ -271,12 +281,12 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
         }
       amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
       amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-      if (kq == 0) amax_l[wn][wm * CM + j * 16 + r16] = __builtin_bit_cast(float, amax);
+      if (kq == 0) amax_l[wn][arow(j) + r16] = __builtin_bit_cast(float, amax);
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < MJ; j++) {
-      const int r = wm * CM + j * 16 + r16;
+    for (int j = 0; j < MC; j++) {
+      const int r = arow(j) + r16;
       if (r >= rows) continue;
       uint32_t amax = 0;
 #pragma unroll
@@ -291,8 +301,8 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < MJ; j++) {
-      const int r = wm * CM + j * 16 + r16;
+    for (int j = 0; j < MC; j++) {
+      const int r = arow(j) + r16;
       if (r >= rows) continue;
 #pragma unroll
       for (int i = 0; i < NI; i++) {
@@ -301,6 +311,12 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
       }
     }
   }
+  };
+  if constexpr (MJ == 8) {
+    if (rows <= 4 * 16 * WM) return body(std::integral_constant<int, 4>{});
+    if (rows <= 6 * 16 * WM) return body(std::integral_constant<int, 6>{});
+  }
+  body(std::integral_constant<int, MJ>{});
 }
 
 template <int DT, bool DUAL, int TN, int TM, int WN, int WM, int NS, bool WIDE>
