@@ -1081,6 +1081,7 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
         *ms = reinterpret_cast<float*>(ws + o_ms);
   hipStream_t st = c->stream;
   mx::BlockGemmArgs gu{}, dn{};
+  gu.splits = dn.splits = 1;
   gu.a = xq; gu.a_s = xs; gu.a_rows = gu.m = T; gu.n = I; gu.k = H; gu.tile_rows = gu_rows;
   gu.c = few ? static_cast<void*>(mid) : mq; gu.c_s = ms;
   gu.w0 = static_cast<const uint8_t*>(w->gate.data); gu.s0 = static_cast<const float*>(w->gate.scales);

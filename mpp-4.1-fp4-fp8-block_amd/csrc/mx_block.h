@@ -76,6 +76,8 @@ struct BlockGemmArgs {
   float* c_s;                        // their scales [n / 128][m]
   int m, n, k;
   int tile_rows;                     // block_tile_rows
+  int splits;                        // parts of K (block_splits): more than one are summed from
+  void* part;                        // f32 [splits][m][n]
   // grouped: row tiles of experts, whose weights lie w_stride and s_stride apart
   const RowTile* tiles;              // null: one matrix
   const int32_t* n_tiles;
@@ -87,6 +89,7 @@ struct BlockGemmArgs {
 // Activation rows of a tile for `rows` rows in `groups` matrices of n rows: 16
 // (weights streamed), 64 or 256.
 int block_tile_rows(long rows, int groups, int n, int c_dtype, bool swiglu);
+int block_splits(int m, int n, int k, int tile_rows);
 // The product by tiles of g.tile_rows rows.  SwiGLU: tiles of 16 rows write f32
 // [m][n] to c, larger ones E4M3 codes to c and their scales to c_s.
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st);

@@ -26,16 +26,16 @@ struct Step {
 
 // 16 NG weight rows (SwiGLU: half of them gate, half up) x 16 activation rows;
 // 4 waves take every fourth 128-block of K, D blocks ahead.
-template <int DT, bool DUAL, int NG, int D>
-__global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
+template <int DT, bool DUAL, int NG, int W, int D>
+__global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
   constexpr int ND = DUAL ? 2 : 1, CH = 16 * NG / ND;  // channels of the workgroup
-  __shared__ float part[4][NG][16][17];
+  __shared__ float part[W][NG][16][17];
   const int NT = (g.n + CH - 1) / CH;
   int row0 = blockIdx.x / NT * 16, rows = min(16, g.m - row0), expert = 0;
   if (g.tiles) {
     const int rt = blockIdx.x / NT;
+    const RowTile t = g.tiles[rt];  // (read beside the count: max_tiles are there)
     if (rt >= *g.n_tiles) return;
-    const RowTile t = g.tiles[rt];
     row0 = t.row0;
     rows = t.rows;
     expert = t.expert;
@@ -73,15 +73,14 @@ __global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
       for (int u = 0; u < 2; u++) s.w[i][u] = *reinterpret_cast<const v4i*>(win ? w[i][u] + o : zeros);
 #pragma unroll
     for (int u = 0; u < 2; u++) s.a[u] = *reinterpret_cast<const v4i*>(kq * 32 + u * 16 < left ? a + o + u * 16 : zeros);
-    const int kc = min(kb, KB - 1);
-    s.as = as[(size_t)kc * g.a_rows];
-    s.ws[0] = s0[kc];
-    if constexpr (DUAL) s.ws[1] = s1[kc];
+    s.as = as[(size_t)kb * g.a_rows];
+    s.ws[0] = s0[kb];
+    if constexpr (DUAL) s.ws[1] = s1[kb];
   };
   v4f acc[NG];
 #pragma unroll
   for (int i = 0; i < NG; i++) acc[i] = v4f{0, 0, 0, 0};
-  auto use = [&](int kb, const Step<NG>& s) {
+  auto use = [&](const Step<NG>& s) {
     v8h x[4];
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -89,7 +88,7 @@ __global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
       for (int h = 0; h < 2; h++) x[2 * u + h] = fp8x8_to_f16<BK_E4M3>((uint32_t)s.a[u][2 * h], (uint32_t)s.a[u][2 * h + 1]);
     float sc[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++) sc[d] = kb < KB ? s.as * s.ws[d] : 0.0f;
+    for (int d = 0; d < ND; d++) sc[d] = s.as * s.ws[d];
 #pragma unroll
     for (int i = 0; i < NG; i++) {
       // lanes of the lower half: row r16 of the first load; upper: of the second
@@ -106,12 +105,13 @@ __global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
   };
   Step<NG> st[D];
 #pragma unroll
-  for (int d = 0; d < D; d++) load(wave + 4 * d, st[d]);
-  for (int kb = wave; kb < KB; kb += 4 * D) {
+  for (int d = 0; d < D; d++)
+    if (wave + W * d < KB) load(wave + W * d, st[d]);
+  for (int kb = wave; kb < KB; kb += W * D) {
 #pragma unroll
     for (int d = 0; d < D; d++) {
-      use(kb + 4 * d, st[d]);
-      load(kb + 4 * (d + D), st[d]);
+      if (kb + W * d < KB) use(st[d]);
+      if (kb + W * (d + D) < KB) load(kb + W * (d + D), st[d]);
     }
   }
 #pragma unroll
@@ -120,14 +120,16 @@ __global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
     for (int v = 0; v < 4; v++) part[wave][i][r16][kq * 4 + v] = acc[i][v];
   __syncthreads();
   // the waves' sums, in their order
-  for (int o = threadIdx.x; o < 16 * CH; o += 256) {
+  for (int o = threadIdx.x; o < 16 * CH; o += 64 * W) {
     const int r = o / CH, c = o % CH;
     if (r >= rows || n0 + c >= g.n) continue;
     float x[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) {
       const int i = c / 16 + d * (NG / 2);
-      x[d] = ((part[0][i][r][c % 16] + part[1][i][r][c % 16]) + part[2][i][r][c % 16]) + part[3][i][r][c % 16];
+      x[d] = part[0][i][r][c % 16];
+#pragma unroll
+      for (int w = 1; w < W; w++) x[d] += part[w][i][r][c % 16];
     }
     float y = x[0];
     if constexpr (DUAL) y = silu(y) * x[1];
@@ -135,23 +137,23 @@ __global__ __launch_bounds__(256) void k_block_stream(BlockGemmArgs g) {
   }
 }
 
-template <int DT, bool DUAL, int NG, int D>
+template <int DT, bool DUAL, int NG, int W, int D>
 hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
   constexpr int CH = 16 * NG / (DUAL ? 2 : 1);
   const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + 15) / 16) * ((g.n + CH - 1) / CH);
   if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_block_stream<DT, DUAL, NG, D>), dim3((unsigned)tiles), dim3(256), 0, st, g);
+  hipLaunchKernelGGL((k_block_stream<DT, DUAL, NG, W, D>), dim3((unsigned)tiles), dim3(64 * W), 0, st, g);
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
-  if (g.w1) return launch_one<MX_DTYPE_F32, true, 2, 4>(g, st);
+  if (g.w1) return launch_one<MX_DTYPE_F32, true, 2, 4, 3>(g, st);
   switch (c_dtype) {
-    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 2, 4>(g, st);
-    case MX_DTYPE_F16: return launch_one<MX_DTYPE_F16, false, 2, 4>(g, st);
-    case MX_DTYPE_BF16: return launch_one<MX_DTYPE_BF16, false, 2, 4>(g, st);
+    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 2, 4, 3>(g, st);
+    case MX_DTYPE_F16: return launch_one<MX_DTYPE_F16, false, 2, 4, 3>(g, st);
+    case MX_DTYPE_BF16: return launch_one<MX_DTYPE_BF16, false, 2, 4, 3>(g, st);
   }
   return hipErrorInvalidValue;
 }

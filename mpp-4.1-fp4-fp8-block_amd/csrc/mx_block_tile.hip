@@ -47,8 +47,9 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   const int NT = (g.n + TN / ND - 1) / (TN / ND), MT = g.tiles ? *g.n_tiles : (g.m + TM - 1) / TM;
   // An XCD takes a run of neighbouring tiles, 8 weight tiles by all row tiles: its
   // 32 CUs then work on about 8 weight and 4 row tiles and fetch each once.
-  const int total = MT * NT, per = (total + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;
+  const int total = MT * NT * g.splits, per = (total + 7) / 8, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || at >= total) return;
+  const int sp = at / (MT * NT), tile = at % (MT * NT);
   const int grp = tile / (8 * MT), in = tile % (8 * MT), gw = min(8, NT - grp * 8);
   const int rt = in / gw, n0 = (grp * 8 + in % gw) * (TN / ND);
   int row0 = rt * TM, rows = min(TM, g.m - row0), expert = 0;
@@ -60,9 +61,10 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
-  const int K = g.k, KB = (K + kQBlock - 1) / kQBlock;
+  // this part's blocks of K: KB from kb0 on
+  const int K = g.k, KA = (K + kQBlock - 1) / kQBlock, kb0 = sp * KA / g.splits, KB = (sp + 1) * KA / g.splits - kb0;
 
-  // block scales of the weights: the whole of K
+  // their scales of the weights
   const size_t so = expert * g.s_stride;
   for (int i = tid; i < KB; i += 64 * NW) {
 #pragma unroll
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
       // SwiGLU: gate and up; else the tile's two blocks of weight rows
       const int nb = n0 / kQBlock + (DUAL ? 0 : d);
       const float* s = (DUAL && d ? g.s1 : g.s0) + so;
-      wsl[d][i] = s[(size_t)min(nb, (g.n - 1) / kQBlock) * KB + i];
+      wsl[d][i] = s[(size_t)min(nb, (g.n - 1) / kQBlock) * KA + kb0 + i];
     }
   }
 
@@ -79,17 +81,17 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   // Through buffer resources of the tile's rows (of a whole batch whose rows are
   // picked): what lies past them reads as zero.  So do chunks past K, on both
   // sides: what lies there may be NaN.
-  const int tail = (K - (KB - 1) * kQBlock) / 16;  // chunks of the last block
+  const int skip = kb0 * kQBlock, tail = min(kQBlock, K - skip - (KB - 1) * kQBlock) / 16;  // chunks of the last block
   const int chunk = (lane & 7) ^ place_key((wave & 1) * 8 + (lane >> 3));
   static_assert(NW % 2 == 0, "a wave's groups of 8 rows are all even or all odd");
   constexpr int TW = TN / ND, QW = TN / 8 / NW, QA = NDMA - QW;  // weight rows of a matrix; instructions of a wave
   static_assert(TN / 8 % NW == 0, "whole instructions");
   // wave w moves weight rows (q NW + w) 8 ..: with SwiGLU, the first half of q gate
-  const uint32_t wrange = (uint32_t)min(TW, g.n - n0) * (uint32_t)K;
-  const size_t wo = expert * g.w_stride + (size_t)n0 * K;
+  const uint32_t wrange = (uint32_t)min(TW, g.n - n0) * (uint32_t)K - skip;
+  const size_t wo = expert * g.w_stride + (size_t)n0 * K + skip;
   const v4i wrs0 = rsrc_of<true>(g.w0 + wo, wrange), wrs1 = rsrc_of<true>((DUAL ? g.w1 : g.w0) + wo, wrange);
   const int woff = (wave * 8 + (lane >> 3)) * K + chunk * 16;
-  const v4i ars = rsrc_of<true>(g.src ? g.a : g.a + (size_t)row0 * K, (uint32_t)(g.src ? g.a_rows : rows) * (uint32_t)K);
+  const v4i ars = rsrc_of<true>((g.src ? g.a : g.a + (size_t)row0 * K) + skip, (uint32_t)(g.src ? g.a_rows : rows) * (uint32_t)K - skip);
   int aoff[QA];
 #pragma unroll
   for (int q = 0; q < QA; q++) {
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
     aoff[q] = r < rows ? (g.src ? g.src[row0 + ra] / g.src_div : ra) * K + chunk * 16 : kPast;
   }
   const int srow = row0 + min((wave * 64) % TM + lane, rows - 1);
-  const float* ssrc = g.a_s + (g.src ? g.src[srow] / g.src_div : srow);
+  const float* ssrc = g.a_s + (size_t)kb0 * g.a_rows + (g.src ? g.src[srow] / g.src_div : srow);
   auto slot = [&](auto u) -> uint8_t* {
     constexpr int U = decltype(u)::value % NS;
     if constexpr (U == 0) return r0;
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int c = n0 + wrow(i) + kq * 4;
-        store4<DT>(g.c, (size_t)(row0 + r) * g.n + c, acc[i][j], g.n - c, g.n % 4 == 0);
+        store4<DT>(g.c, ((size_t)sp * g.m + row0 + r) * g.n + c, acc[i][j], g.n - c, g.n % 4 == 0);
       }
     }
   }
@@ -319,25 +321,67 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   body(std::integral_constant<int, MJ>{});
 }
 
+// Sums of a product's parts, in their order.
+template <int DT, int N>
+__global__ __launch_bounds__(256) void k_block_join(const float* part, size_t len, int splits, void* c) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * N;
+  if (i >= len) return;
+  float sum[N], v[N];
+  load_n_as_f32<MX_DTYPE_F32, N>(part, i, sum);
+  for (int s = 1; s < splits; s++) {
+    load_n_as_f32<MX_DTYPE_F32, N>(part, s * len + i, v);
+#pragma unroll
+    for (int u = 0; u < N; u++) sum[u] += v[u];
+  }
+  store_n_from_f32<DT, N>(c, i, sum);
+}
+
 template <int DT, bool DUAL, int TN, int TM, int WN, int WM, int NS, bool WIDE>
 hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
   const int nt = (g.n + TN / (DUAL ? 2 : 1) - 1) / (TN / (DUAL ? 2 : 1));
-  const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + TM - 1) / TM) * nt;
+  const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + TM - 1) / TM) * nt * g.splits;
   if (tiles > 0x7ffffff0L) return hipErrorInvalidValue;
   hipLaunchKernelGGL((k_block_tile<DT, DUAL, TN, TM, WN, WM, NS, WIDE>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
                      st, g);
   return hipGetLastError();
 }
 
+template <int DT>
+hipError_t store_tiles(const BlockGemmArgs& g, hipStream_t st) {
+  if constexpr (DT != MX_DTYPE_F32) {
+    if (g.tile_rows == 256) return launch_one<DT, false, 256, 256, 4, 2, 2, false>(g, st);
+  }
+  if (g.splits == 1) return launch_one<DT, false, 128, 64, 4, 1, 3, true>(g, st);
+  BlockGemmArgs p = g;
+  p.c = g.part;
+  if (hipError_t e = launch_one<MX_DTYPE_F32, false, 128, 64, 4, 1, 3, true>(p, st)) return e;
+  const size_t len = (size_t)g.m * g.n;
+  const float* part = static_cast<const float*>(g.part);
+  if (len % 8 == 0) hipLaunchKernelGGL((k_block_join<DT, 8>), dim3((unsigned)((len / 8 + 255) / 256)), dim3(256), 0, st, part, len, g.splits, g.c);
+  else hipLaunchKernelGGL((k_block_join<DT, 1>), dim3((unsigned)((len + 255) / 256)), dim3(256), 0, st, part, len, g.splits, g.c);
+  return hipGetLastError();
+}
+
 }  // namespace
 
+// Parts of K for a dense product by 64-row tiles: about two workgroups a CU,
+// each with four blocks at least.
+int block_splits(int m, int n, int k, int tile_rows) {
+  if (tile_rows != 64) return 1;
+  const long tiles = (long)((m + 63) / 64) * ((n + 127) / 128);
+  const int kb = (k + kQBlock - 1) / kQBlock;
+  const long s = 512 / tiles;
+  return s <= 1 ? 1 : s > kb / 4 ? (kb / 4 > 1 ? kb / 4 : 1) : (int)s;
+}
+
 hipError_t launch_block_tile(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
-  const int side = g.tile_rows;
-  if (g.w1) return side == 256 ? launch_one<MX_DTYPE_F32, true, 256, 256, 4, 2, 2, false>(g, st) : launch_one<MX_DTYPE_F32, true, 256, 64, 8, 1, 3, true>(g, st);
+  if (g.w1)
+    return g.tile_rows == 256 ? launch_one<MX_DTYPE_F32, true, 256, 256, 4, 2, 2, false>(g, st)
+                              : launch_one<MX_DTYPE_F32, true, 256, 64, 8, 1, 3, true>(g, st);
   switch (c_dtype) {
-    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 128, 64, 4, 1, 3, true>(g, st);
-    case MX_DTYPE_F16: return side == 256 ? launch_one<MX_DTYPE_F16, false, 256, 256, 4, 2, 2, false>(g, st) : launch_one<MX_DTYPE_F16, false, 128, 64, 4, 1, 3, true>(g, st);
-    case MX_DTYPE_BF16: return side == 256 ? launch_one<MX_DTYPE_BF16, false, 256, 256, 4, 2, 2, false>(g, st) : launch_one<MX_DTYPE_BF16, false, 128, 64, 4, 1, 3, true>(g, st);
+    case MX_DTYPE_F32: return store_tiles<MX_DTYPE_F32>(g, st);
+    case MX_DTYPE_F16: return store_tiles<MX_DTYPE_F16>(g, st);
+    case MX_DTYPE_BF16: return store_tiles<MX_DTYPE_BF16>(g, st);
   }
   return hipErrorInvalidValue;
 }

@@ -90,6 +90,7 @@ int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x
   g.tiles = d.tiles;
   g.n_tiles = d.n_tiles;
   g.max_tiles = max_tiles;
+  g.splits = 1;
   g.tile_rows = tile_rows;
   g.w_stride = (size_t)I * H;
   g.s_stride = (size_t)blocks(I) * blocks(H);
@@ -233,6 +234,9 @@ int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const ui
   g.n = n;
   g.k = k;
   g.tile_rows = mx::block_tile_rows(m, 1, n, c_dtype, false);
+  g.splits = mx::block_splits(m, n, k, g.tile_rows);
+  if (g.splits > 1)
+    if (int rc = mx_ctx_workspace(c, (size_t)g.splits * m * n * 4, &g.part)) return rc;
   MX_RUN(c, mx::launch_block_gemm(c_dtype, g, mx_ctx_stream(c)));
   return MX_OK;
 }
