@@ -12,6 +12,7 @@ namespace mx {
 
 constexpr int kQBlock = 128;         // values (of weights: rows too) of one block scale
 constexpr int kMaxBlocks = 512;       // blocks of K in one product
+constexpr int kMaxDirect = 8192;      // values of a row that launch_block_direct quantizes
 constexpr int kMaxRouteExperts = 512;
 constexpr int kMaxRouteGroups = 64;
 
@@ -45,9 +46,11 @@ struct DispatchArgs {
 };
 size_t dispatch_ws_bytes(int n, int experts);
 hipError_t launch_dispatch(const DispatchArgs& a, hipStream_t st);
-// xs[rows[t][s]] = x[t]; row_bytes of any size
-hipError_t launch_gather(const void* x, const int32_t* rows, void* xs, int tokens, int topk, size_t row_bytes,
-                         hipStream_t st);
+// and xs[rows[t][s]] = x[t]; row_bytes of any even size
+hipError_t launch_dispatch_rows(const DispatchArgs& a, int topk, const void* x, void* xs, size_t row_bytes, hipStream_t st);
+// and x (f16 or bf16) as launch_block_quantize does
+hipError_t launch_prepare(const DispatchArgs& a, int dtype, const void* x, int rows, int k, uint8_t* q, float* scales,
+                          hipStream_t st);
 
 struct CombineArgs {
   const void* y;
@@ -56,6 +59,9 @@ struct CombineArgs {
   const void* add;                   // null: none
   void* out;
   int tokens, topk, hidden;
+  // rows null: the row of a slot is the slot, where its expert is one of `experts`
+  const int32_t* ids;
+  int experts;
 };
 hipError_t launch_combine(int y_dtype, int out_dtype, const CombineArgs& a, hipStream_t st);
 
@@ -85,6 +91,11 @@ struct BlockGemmArgs {
   size_t w_stride, s_stride;
   const int32_t* src;                // row -> slot, and
   int src_div;                       // slot / src_div = row of a (null: row of a = row)
+  // one token's slots (launch_block_direct): the row is quantized where it is used
+  const void* raw;                   // [k], or [m][k] with row_per_slot
+  int row_per_slot;
+  const int32_t* ids;                // [m] the slots' experts
+  int experts;
 };
 // Activation rows of a tile for `rows` rows in `groups` matrices of n rows: 16
 // (weights streamed), 64 or 256.
@@ -94,6 +105,9 @@ int block_splits(int m, int n, int k, int tile_rows);
 // [m][n] to c, larger ones E4M3 codes to c and their scales to c_s.
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st);
 hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st);  // mx_block_stream.hip
+// One token, k <= kMaxDirect: gate/up products of an f16 or bf16 row or the down
+// product of its f32 middles, to f32.
+hipError_t launch_block_direct(int raw_dtype, const BlockGemmArgs& g, hipStream_t st);
 hipError_t launch_block_tile(int c_dtype, const BlockGemmArgs& g, hipStream_t st);    // mx_block_tile.hip
 
 }  // namespace mx

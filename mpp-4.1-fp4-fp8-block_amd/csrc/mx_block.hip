@@ -5,23 +5,13 @@
 namespace mx {
 namespace {
 
-// 16 lanes of 8 values a block; a workgroup takes 16 rows, so that their
-// scales are written together.
+// Bound: HBM and L2 (34 MB of bf16 at 3.5 TB/s, read and written).  A workgroup
+// takes one block of 16 rows, so that their scales are written together; four
+// blocks a lane, all loaded first, measured 14.3 -> 17.4 us.
 template <int DT>
 __global__ __launch_bounds__(256) void k_quantize(const void* src, int rows, int k, uint8_t* q, float* scales) {
-  const int lane16 = threadIdx.x & 15, row = blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  const int kb = blockIdx.y, at = kb * kQBlock + lane16 * 8;
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (at < k) load_n_as_f32<DT, 8>(src, (size_t)row * k + at, v);
-  uint32_t amax = 0;
-#pragma unroll
-  for (int u = 0; u < 8; u++) amax = max(amax, abs_bits(v[u]));
-#pragma unroll
-  for (int o = 8; o; o >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, o));
-  const float s = block_scale(amax);
-  if (at < k) *reinterpret_cast<v2i*>(q + (size_t)row * k + at) = v2i{(int)e4m3x4(v4f{v[0], v[1], v[2], v[3]}, s), (int)e4m3x4(v4f{v[4], v[5], v[6], v[7]}, s)};
-  if (lane16 == 0) scales[(size_t)kb * rows + row] = s;
+  const int row = blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (row < rows) quantize_block<DT>(src, rows, k, q, scales, row, blockIdx.y);
 }
 
 // One workgroup per 128 x 128 block, 64 values a thread.

@@ -24,6 +24,28 @@ __device__ __forceinline__ uint32_t e4m3x4(v4f v, float s) {
   return __builtin_bit_cast(uint32_t, w);
 }
 
+// 16 lanes quantize one block of a row, 8 values each (v: the lane's, 0 past the
+// row); returns its scale, and writes the codes to q unless it is null.
+__device__ __forceinline__ float quantize_lanes16(const float* v, uint8_t* q) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int u = 0; u < 8; u++) amax = max(amax, abs_bits(v[u]));
+#pragma unroll
+  for (int o = 8; o; o >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, o));
+  const float s = block_scale(amax);
+  if (q) *reinterpret_cast<v2i*>(q) = v2i{(int)e4m3x4(v4f{v[0], v[1], v[2], v[3]}, s), (int)e4m3x4(v4f{v[4], v[5], v[6], v[7]}, s)};
+  return s;
+}
+
+template <int DT>
+__device__ __forceinline__ void quantize_block(const void* src, int rows, int k, uint8_t* q, float* scales, int row, int kb) {
+  const int c = kb * kQBlock + (threadIdx.x & 15) * 8;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (c < k) load_n_as_f32<DT, 8>(src, (size_t)row * k + c, v);
+  const float s = quantize_lanes16(v, c < k ? q + (size_t)row * k + c : nullptr);
+  if ((threadIdx.x & 15) == 0) scales[(size_t)kb * rows + row] = s;
+}
+
 // The sum of one 128-block of 16 weight rows (the MFMA's rows) and 16 activation
 // rows (its columns): a lane has one activation scale and one weight scale for
 // its four sums, and four neighbouring outputs.  Both operands hold byte j of

@@ -25,14 +25,35 @@ struct Step {
 };
 
 // 16 NG weight rows (SwiGLU: half of them gate, half up) x 16 activation rows;
-// 4 waves take every fourth 128-block of K, D blocks ahead.
-template <int DT, bool DUAL, int NG, int W, int D>
+// W waves take every W-th 128-block of K, D blocks ahead.  XT >= 0: one token, whose
+// slots are the row tiles; the workgroup quantizes its row (in XT) into LDS while
+// its first weights are on their way.
+template <int DT, bool DUAL, int NG, int W, int D, int XT>
 __global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
   constexpr int ND = DUAL ? 2 : 1, CH = 16 * NG / ND;  // channels of the workgroup
+  constexpr bool RAW = XT >= 0;
   __shared__ float part[W][NG][16][17];
+  __shared__ __attribute__((aligned(16))) uint8_t xq[RAW ? kMaxDirect : 16];
+  __shared__ float xs[RAW ? kMaxDirect / kQBlock : 1];
   const int NT = (g.n + CH - 1) / CH;
   int row0 = blockIdx.x / NT * 16, rows = min(16, g.m - row0), expert = 0;
-  if (g.tiles) {
+  // (the row's values are under way before the slot's expert is known)
+  constexpr int RB = RAW ? kMaxDirect / kQBlock / (4 * W) : 1;
+  float raw[RB][8];
+  if constexpr (RAW) {
+    row0 = blockIdx.x / NT;
+    rows = 1;
+    const size_t at = (size_t)(g.row_per_slot ? row0 : 0) * g.k;
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      const int c = (i * 64 * W + threadIdx.x) * 8;  // block i * 4 W + tid / 16
+#pragma unroll
+      for (int u = 0; u < 8; u++) raw[i][u] = 0.0f;
+      if (c < g.k) load_n_as_f32<RAW ? XT : MX_DTYPE_F32, 8>(g.raw, at + c, raw[i]);
+    }
+    expert = g.ids[row0];
+    if ((unsigned)expert >= (unsigned)g.experts) return;
+  } else if (g.tiles) {
     const int rt = blockIdx.x / NT;
     const RowTile t = g.tiles[rt];  // (read beside the count: max_tiles are there)
     if (rt >= *g.n_tiles) return;
@@ -55,7 +76,7 @@ __global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
       const int n = n0 + (i % (NG / ND)) * 16 + u * 8 + (r16 & 7);
       w[i][u] = (DUAL && i >= NG / 2 ? g.w1 : g.w0) + expert * g.w_stride + (size_t)min(n, g.n - 1) * K + wchunk * 16;
     }
-  const int row = row0 + min(r16, rows - 1), ar = g.src ? g.src[row] / g.src_div : row;
+  const int row = row0 + min(r16, rows - 1), ar = RAW ? 0 : g.src ? g.src[row] / g.src_div : row;
   const uint8_t* a = g.a + (size_t)ar * K + kq * 32;
   const float* as = g.a_s + ar;
   const size_t so = expert * g.s_stride + (size_t)(n0 / kQBlock) * KB;
@@ -71,24 +92,27 @@ __global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
     for (int i = 0; i < NG; i++)
 #pragma unroll
       for (int u = 0; u < 2; u++) s.w[i][u] = *reinterpret_cast<const v4i*>(win ? w[i][u] + o : zeros);
+    s.ws[0] = s0[kb];
+    if constexpr (DUAL) s.ws[1] = s1[kb];
+    if constexpr (RAW) return;
 #pragma unroll
     for (int u = 0; u < 2; u++) s.a[u] = *reinterpret_cast<const v4i*>(kq * 32 + u * 16 < left ? a + o + u * 16 : zeros);
     s.as = as[(size_t)kb * g.a_rows];
-    s.ws[0] = s0[kb];
-    if constexpr (DUAL) s.ws[1] = s1[kb];
   };
   v4f acc[NG];
 #pragma unroll
   for (int i = 0; i < NG; i++) acc[i] = v4f{0, 0, 0, 0};
-  auto use = [&](const Step<NG>& s) {
+  auto use = [&](int kb, const Step<NG>& s) {
     v8h x[4];
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int u = 0; u < 2; u++) {
+      const v4i codes = RAW ? *reinterpret_cast<const v4i*>(xq + kb * kQBlock + kq * 32 + u * 16) : s.a[u];
 #pragma unroll
-      for (int h = 0; h < 2; h++) x[2 * u + h] = fp8x8_to_f16<BK_E4M3>((uint32_t)s.a[u][2 * h], (uint32_t)s.a[u][2 * h + 1]);
+      for (int h = 0; h < 2; h++) x[2 * u + h] = fp8x8_to_f16<BK_E4M3>((uint32_t)codes[2 * h], (uint32_t)codes[2 * h + 1]);
+    }
     float sc[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++) sc[d] = s.as * s.ws[d];
+    for (int d = 0; d < ND; d++) sc[d] = (RAW ? xs[kb] : s.as) * s.ws[d];
 #pragma unroll
     for (int i = 0; i < NG; i++) {
       // lanes of the lower half: row r16 of the first load; upper: of the second
@@ -107,10 +131,20 @@ __global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
 #pragma unroll
   for (int d = 0; d < D; d++)
     if (wave + W * d < KB) load(wave + W * d, st[d]);
+  if constexpr (RAW) {
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      const int kb = i * 4 * W + (threadIdx.x >> 4);
+      if (kb >= KB) break;
+      const float sc = quantize_lanes16(raw[i], xq + kb * kQBlock + (threadIdx.x & 15) * 8);
+      if ((threadIdx.x & 15) == 0) xs[kb] = sc;
+    }
+    __syncthreads();
+  }
   for (int kb = wave; kb < KB; kb += W * D) {
 #pragma unroll
     for (int d = 0; d < D; d++) {
-      if (kb + W * d < KB) use(st[d]);
+      if (kb + W * d < KB) use(kb + W * d, st[d]);
       if (kb + W * (d + D) < KB) load(kb + W * (d + D), st[d]);
     }
   }
@@ -120,9 +154,9 @@ __global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
     for (int v = 0; v < 4; v++) part[wave][i][r16][kq * 4 + v] = acc[i][v];
   __syncthreads();
   // the waves' sums, in their order
-  for (int o = threadIdx.x; o < 16 * CH; o += 64 * W) {
+  for (int o = threadIdx.x; o < rows * CH; o += 64 * W) {
     const int r = o / CH, c = o % CH;
-    if (r >= rows || n0 + c >= g.n) continue;
+    if (n0 + c >= g.n) continue;
     float x[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) {
@@ -137,23 +171,35 @@ __global__ __launch_bounds__(64 * W) void k_block_stream(BlockGemmArgs g) {
   }
 }
 
-template <int DT, bool DUAL, int NG, int W, int D>
+template <int DT, bool DUAL, int NG, int W, int D, int XT>
 hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
   constexpr int CH = 16 * NG / (DUAL ? 2 : 1);
-  const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + 15) / 16) * ((g.n + CH - 1) / CH);
+  const long tiles = (long)(XT >= 0 ? g.m : g.tiles ? g.max_tiles : (g.m + 15) / 16) * ((g.n + CH - 1) / CH);
   if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_block_stream<DT, DUAL, NG, W, D>), dim3((unsigned)tiles), dim3(64 * W), 0, st, g);
+  hipLaunchKernelGGL((k_block_stream<DT, DUAL, NG, W, D, XT>), dim3((unsigned)tiles), dim3(64 * W), 0, st, g);
   return hipGetLastError();
+}
+
+template <int XT>
+hipError_t launch_any(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
+  if (g.w1) return launch_one<MX_DTYPE_F32, true, 2, 4, 3, XT>(g, st);
+  switch (c_dtype) {
+    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 2, 4, 3, XT>(g, st);
+    case MX_DTYPE_F16: return launch_one<MX_DTYPE_F16, false, 2, 4, 3, XT>(g, st);
+    case MX_DTYPE_BF16: return launch_one<MX_DTYPE_BF16, false, 2, 4, 3, XT>(g, st);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
-  if (g.w1) return launch_one<MX_DTYPE_F32, true, 2, 4, 3>(g, st);
-  switch (c_dtype) {
-    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 2, 4, 3>(g, st);
-    case MX_DTYPE_F16: return launch_one<MX_DTYPE_F16, false, 2, 4, 3>(g, st);
-    case MX_DTYPE_BF16: return launch_one<MX_DTYPE_BF16, false, 2, 4, 3>(g, st);
+hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st) { return launch_any<-1>(c_dtype, g, st); }
+
+hipError_t launch_block_direct(int raw_dtype, const BlockGemmArgs& g, hipStream_t st) {
+  switch (raw_dtype) {
+    case MX_DTYPE_F32: return launch_one<MX_DTYPE_F32, false, 2, 4, 3, MX_DTYPE_F32>(g, st);  // the middle
+    case MX_DTYPE_F16: return launch_one<MX_DTYPE_F32, true, 2, 4, 3, MX_DTYPE_F16>(g, st);
+    case MX_DTYPE_BF16: return launch_one<MX_DTYPE_F32, true, 2, 4, 3, MX_DTYPE_BF16>(g, st);
   }
   return hipErrorInvalidValue;
 }

@@ -1,11 +1,44 @@
 // mx_moe.hip - the router of a mixture of experts, and the exchange of rows
 // between token order and expert order.
-#include "mx_block.h"
-#include "mx_convert.h"
-#include "mx_device.h"
+#include "mx_block_device.h"
 
 namespace mx {
 namespace {
+
+// ---- lanes ----------------------------------------------------------------------
+// DPP: lane ^ 1, lane ^ 2, 7 - lane of 8, 15 - lane of 16.  After as many of them as
+// log2(L), every lane of L has what the L lanes have together.
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) { return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v))); }
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)dpp<CTRL>((uint32_t)(u >> 32)) << 32 | dpp<CTRL>((uint32_t)u));
+}
+template <class T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(T, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane) << 32 |
+                                     (uint32_t)__builtin_amdgcn_readlane((int)u, lane));
+  } else {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  }
+}
+// op over the wave's 64 lanes, as a uniform value
+template <class T, class Op>
+__device__ __forceinline__ T over_wave(T v, Op op) {
+  v = op(v, dpp<kXor1>(v));
+  v = op(v, dpp<kXor2>(v));
+  v = op(v, dpp<kMirror8>(v));
+  v = op(v, dpp<kMirror16>(v));
+  return op(op(lane_value(v, 0), lane_value(v, 16)), op(lane_value(v, 32), lane_value(v, 48)));
+}
 
 // ---- router ---------------------------------------------------------------------
 //
@@ -15,6 +48,12 @@ namespace {
 // One wave a token, expert j * 64 + lane in register j.  The sum of a softmax is
 // taken in f64 and rounded once, so that keys, and with them the choice, do not
 // depend on the order of the sum.
+//
+// Bound: instructions, and at few tokens the launch.  The maximum of a wave by
+// DPP and four lane reads, then the holder by one comparison a register, is a third
+// of the instructions of a 64-bit (key, index) maximum by lane shuffles.
+
+// Keys as integers of the same order; 0: not available.
 __device__ __forceinline__ uint32_t ordered(float f) {
   const uint32_t u = __builtin_bit_cast(uint32_t, f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -23,17 +62,21 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 template <int DT, int NP>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
   __shared__ float keys[4][NP * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = blockIdx.x * 4 + wave;
   if (t >= a.tokens) return;
   const float kLow = -__builtin_inff(), kTop = 3.402823466e38f;
   const int E = a.experts;
   float v[NP], p[NP], key[NP];
-  float top = -kTop;
 #pragma unroll
   for (int j = 0; j < NP; j++) {
     const int e = j * 64 + lane;
     v[j] = e < E ? load_as_f32<DT>(a.logits, (size_t)t * a.stride + e) : kLow;
+    key[j] = a.bias && e < E ? a.bias[e] : 0.0f;
+  }
+  float top = -kTop;
+#pragma unroll
+  for (int j = 0; j < NP; j++) {
     if (!(v[j] > kLow)) v[j] = kLow;  // NaN: masked
     v[j] = fminf(v[j], kTop);
     top = fmaxf(top, v[j]);
@@ -42,77 +85,85 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
 #pragma unroll
     for (int j = 0; j < NP; j++) p[j] = 1.0f / (1.0f + expf(-v[j]));
   } else {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = over_wave(top, [](float x, float y) { return fmaxf(x, y); });
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < NP; j++) {
       p[j] = v[j] > kLow ? expf(v[j] - top) : 0.0f;
       sum += (double)p[j];
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    const float s = (float)sum;
+    const float s = (float)over_wave(sum, [](double x, double y) { return x + y; });
 #pragma unroll
     for (int j = 0; j < NP; j++) p[j] = p[j] / s;
   }
 #pragma unroll
   for (int j = 0; j < NP; j++) {
-    const int e = j * 64 + lane;
-    key[j] = a.bias && e < E ? p[j] + a.bias[e] : p[j];
+    key[j] = p[j] + key[j];
     if (!(v[j] > kLow) || !(key[j] > kLow)) key[j] = kLow;
   }
   if (a.groups > 1) {
-    const int size = E / a.groups;
+    // L lanes a group; the first one keeps its score
+    const int size = E / a.groups, L = 64 >> (32 - __builtin_clz(a.groups - 1)), sub = lane & (L - 1), grp = lane / L;
 #pragma unroll
     for (int j = 0; j < NP; j++) keys[wave][j * 64 + lane] = key[j];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     float b0 = kLow, b1 = kLow;
-    if (lane < a.groups)
-      for (int i = 0; i < size; i++) {
-        const float k = keys[wave][lane * size + i];
+    if (grp < a.groups)
+      for (int i = sub; i < size; i += L) {
+        const float k = keys[wave][grp * size + i];
         b1 = fmaxf(b1, fminf(k, b0));
         b0 = fmaxf(b0, k);
       }
+    auto join = [&](float o0, float o1) {
+      b1 = fmaxf(fminf(b0, o0), fmaxf(b1, o1));
+      b0 = fmaxf(b0, o0);
+    };
+    if (L >= 2) join(dpp<kXor1>(b0), dpp<kXor1>(b1));
+    if (L >= 4) join(dpp<kXor2>(b0), dpp<kXor2>(b1));
+    if (L >= 8) join(dpp<kMirror8>(b0), dpp<kMirror8>(b1));
+    if (L >= 16) join(dpp<kMirror16>(b0), dpp<kMirror16>(b1));
+    if (L >= 32) join(__shfl_xor(b0, 16), __shfl_xor(b1, 16));
     const float score = a.group_top == 2 && b1 > kLow ? b0 + b1 : b0;
     int rank = 0;
     for (int i = 0; i < a.groups; i++) {
-      const float s = __shfl(score, i);
-      rank += s > score || (s == score && i < lane);
+      const float s = lane_value(score, i * L);
+      rank += s > score || (s == score && i < grp);
     }
-    const uint64_t kept = __ballot(lane < a.groups && rank < a.topk_groups);
+    const uint64_t kept = __ballot(grp < a.groups && rank < a.topk_groups);
+    const float per = 1.0f / (float)size;  // (e + 0.5) / size is at least 0.5 / size from a whole number
 #pragma unroll
     for (int j = 0; j < NP; j++) {
-      const int e = j * 64 + lane;
-      if (e < E && !((kept >> (e / size)) & 1)) key[j] = kLow;
+      const int e = j * 64 + lane, ge = (int)(((float)e + 0.5f) * per);
+      if (e < E && !((kept >> (ge * L)) & 1)) key[j] = kLow;
     }
   }
   // best first; the lower index wins a tie
+  uint32_t ord[NP];
+#pragma unroll
+  for (int j = 0; j < NP; j++) ord[j] = key[j] > kLow ? ordered(key[j]) : 0;
   float mine = 0.0f, total = 0.0f;
   int id = -1;
   for (int s = 0; s < a.topk; s++) {
-    uint64_t best = 0;
+    uint32_t best = ord[0];
 #pragma unroll
-    for (int j = 0; j < NP; j++) {
-      const uint64_t c = key[j] > kLow ? (uint64_t)ordered(key[j]) << 32 | (uint32_t)(0xffff - (j * 64 + lane)) : 0;
-      best = c > best ? c : best;
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-      const uint64_t c = __shfl_xor((unsigned long long)best, o);
-      best = c > best ? c : best;
-    }
+    for (int j = 1; j < NP; j++) best = max(best, ord[j]);
+    best = over_wave(best, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
     if (!best) break;
-    const int e = 0xffff - (int)(best & 0xffffffffu);
     float w = 0.0f;
+    int e = -1;
+#pragma unroll
+    for (int j = NP - 1; j >= 0; j--) {
+      const uint64_t at = __ballot(ord[j] == best);
+      if (at) {
+        const int l = __builtin_ctzll(at);
+        e = j * 64 + l;
+        w = lane_value(p[j], l);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NP; j++)
-      if (j == e >> 6) w = p[j];
-    w = __shfl(w, e & 63);
-#pragma unroll
-    for (int j = 0; j < NP; j++)
-      if (j * 64 + lane == e) key[j] = kLow;
+      if (j * 64 + lane == e) ord[j] = 0;
     total += w;
     if (lane == s) { mine = w; id = e; }
   }
@@ -136,32 +187,35 @@ hipError_t route_dt(const RouteArgs& a, hipStream_t st) {
 }
 
 // ---- expert order -----------------------------------------------------------------
-// A stable counting sort of the slots by expert, in chunks of kChunk slots: the
-// chunks' histograms, then every chunk adds up those before it and gives its
-// slots their rows.  A wave finds the slots of one expert among its 64 by nine
-// ballots, one a bit; only integer counts are added by atomics, so the order
-// of the rows is the slots'.
-constexpr int kChunk = 2048, kPerWave = kChunk / 4;
+// A stable counting sort of the slots by expert.  A workgroup places kChunk slots:
+// it needs the counts of all slots before and after them, which it takes from all
+// ids where those are few (one launch; 32768 of them cost 2 us) and from a table of
+// the chunks' counts, written by a launch of its own, where they are many.  A wave
+// finds the slots of one expert among its 64 by nine ballots, one a bit; only
+// integer counts are added by atomics, so the order of the rows is the slots'.
+constexpr int kPlaceThreads = 1024, kPlaceWaves = kPlaceThreads / 64, kChunk = 4096, kPerWave = kChunk / kPlaceWaves;
+constexpr int kCopies = 4;
+constexpr int kMaxCounted = 16 * kChunk;  // ids that every workgroup counts itself
 
 __device__ __forceinline__ int expert_of(const DispatchArgs& a, int i) {
   const int e = i < a.n ? a.ids[i] : -1;
   return (unsigned)e < (unsigned)a.experts ? e : -1;
 }
 
-__global__ __launch_bounds__(256) void k_count(DispatchArgs a) {
+__global__ __launch_bounds__(kPlaceThreads) void k_count(DispatchArgs a) {
   __shared__ int h[kMaxRouteExperts];
-  for (int e = threadIdx.x; e < a.experts; e += 256) h[e] = 0;
+  for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) h[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < kChunk; i += 256) {
+  for (int i = threadIdx.x; i < kChunk; i += kPlaceThreads) {
     const int e = expert_of(a, blockIdx.x * kChunk + i);
     if (e >= 0) atomicAdd(&h[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.experts; e += 256) a.hist[(size_t)blockIdx.x * a.experts + e] = h[e];
+  for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) a.hist[(size_t)blockIdx.x * a.experts + e] = h[e];
 }
 
-// inclusive prefix sums of v over the workgroup's 256 threads
-__device__ __forceinline__ int scan256(int v, int* part) {
+// inclusive prefix sums of v over the workgroup's threads
+__device__ __forceinline__ int scan_all(int v, int* part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -175,72 +229,81 @@ __device__ __forceinline__ int scan256(int v, int* part) {
   return v;
 }
 
-__global__ __launch_bounds__(256) void k_place(DispatchArgs a, int chunks) {
-  __shared__ int at[4][kMaxRouteExperts];   // next row of an expert, by wave
-  __shared__ int part[4];
+struct PlaceShared {
+  int at[kPlaceWaves][kMaxRouteExperts];  // next row of an expert, by wave
+  int other[2][kCopies][kMaxRouteExperts];  // slots before the chunk, and after it
+  int part[kPlaceWaves];
+};
+
+// chunk `chunk` of the slots, by kPlaceThreads threads
+__device__ __forceinline__ void place(const DispatchArgs& a, int chunk, PlaceShared& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.experts;
-  const int first = blockIdx.x * kChunk + wave * kPerWave;
-  for (int i = tid; i < 4 * kMaxRouteExperts; i += 256) at[0][i] = 0;
+  const int first = chunk * kChunk, mine0 = first + wave * kPerWave;
+  for (int i = tid; i < kPlaceWaves * kMaxRouteExperts; i += kPlaceThreads) s.at[0][i] = 0;
+  for (int i = tid; i < 2 * kCopies * kMaxRouteExperts; i += kPlaceThreads) s.other[0][0][i] = 0;
   __syncthreads();
   int mine[kPerWave / 64];
 #pragma unroll
-  for (int i = 0; i < kPerWave / 64; i++) {
-    mine[i] = expert_of(a, first + i * 64 + lane);
-    if (mine[i] >= 0) atomicAdd(&at[wave][mine[i]], 1);
+  for (int i = 0; i < kPerWave / 64; i++) mine[i] = expert_of(a, mine0 + i * 64 + lane);
+  if (a.hist) {
+    const int chunks = (a.n + kChunk - 1) / kChunk;
+    if (tid < E)
+      for (int c = 0; c < chunks; c++)
+        if (c != chunk) s.other[c > chunk][0][tid] += a.hist[(size_t)c * E + tid];
+  } else {
+    // eight loads at a time; the lanes' counts are spread over copies, since lanes
+    // that add to one word take turns
+    constexpr int kAhead = 8;
+    int* copy = s.other[0][tid & (kCopies - 1)];
+    for (int i0 = tid; i0 < a.n; i0 += kAhead * kPlaceThreads) {
+      int e[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) e[u] = expert_of(a, i0 + u * kPlaceThreads);
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const int c = (i0 + u * kPlaceThreads) / kChunk;
+        if (e[u] >= 0 && c != chunk) atomicAdd(copy + (c > chunk ? kCopies * kMaxRouteExperts : 0) + e[u], 1);
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < kPerWave / 64; i++)
+    if (mine[i] >= 0) atomicAdd(&s.at[wave][mine[i]], 1);
   __syncthreads();
-  // experts 2 tid and 2 tid + 1
-  int before[2] = {0, 0}, all[2] = {0, 0};
+  int own = 0, before = 0, all = 0;
+  if (tid < E) {
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const int e = 2 * tid + u;
-    if (e >= E) continue;
-    if (chunks == 1) {
-      all[u] = at[0][e] + at[1][e] + at[2][e] + at[3][e];
-    } else {
-      for (int c = 0; c < chunks; c++) {
-        const int h = a.hist[(size_t)c * E + e];
-        all[u] += h;
-        if (c < (int)blockIdx.x) before[u] += h;
-      }
+    for (int w = 0; w < kPlaceWaves; w++) own += s.at[w][tid];
+    all = own;
+#pragma unroll
+    for (int c = 0; c < kCopies; c++) {
+      before += s.other[0][c][tid];
+      all += s.other[0][c][tid] + s.other[1][c][tid];
     }
   }
-  const int incl = scan256(all[0] + all[1], part);
-  const int start[2] = {incl - all[0] - all[1], incl - all[1]};
-  if (blockIdx.x == 0) {
-    int tiles[2] = {0, 0};
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-      if (2 * tid + u < E) {
-        a.counts[2 * tid + u] = all[u];
-        if (a.tiles) tiles[u] = (all[u] + a.tile_rows - 1) / a.tile_rows;
-      }
+  const int start = scan_all(all, s.part) - all;
+  if (chunk == 0) {
+    if (tid < E) a.counts[tid] = all;
     if (a.tiles) {
-      const int ti = scan256(tiles[0] + tiles[1], part);
-      if (tid == 255) *a.n_tiles = ti;
-      int next = ti - tiles[0] - tiles[1];
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-        for (int i = 0; i < tiles[u]; i++)
-          a.tiles[next++] = RowTile{2 * tid + u, start[u] + i * a.tile_rows, min(a.tile_rows, all[u] - i * a.tile_rows), 0};
+      const int tiles = (all + a.tile_rows - 1) / a.tile_rows, end = scan_all(tiles, s.part);
+      if (tid == kPlaceThreads - 1) *a.n_tiles = end;
+      for (int i = 0; i < tiles; i++)
+        a.tiles[end - tiles + i] = RowTile{tid, start + i * a.tile_rows, min(a.tile_rows, all - i * a.tile_rows), 0};
     }
   }
+  if (tid < E) {
+    int row = start + before;
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const int e = 2 * tid + u;
-    if (e >= E) continue;
-    int row = start[u] + before[u];
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const int c = at[w][e];
-      at[w][e] = row;
+    for (int w = 0; w < kPlaceWaves; w++) {
+      const int c = s.at[w][tid];
+      s.at[w][tid] = row;
       row += c;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPerWave / 64; i++) {
-    const int slot = first + i * 64 + lane, e = mine[i];
+    const int slot = mine0 + i * 64 + lane, e = mine[i];
     uint64_t same = __ballot(e >= 0);
 #pragma unroll
     for (int b = 0; b < 9; b++) {
@@ -253,11 +316,77 @@ __global__ __launch_bounds__(256) void k_place(DispatchArgs a, int chunks) {
       // their order
       const int lead = __builtin_ctzll(same);
       int base = 0;
-      if (lane == lead) base = atomicAdd(&at[wave][e], (int)__builtin_popcountll(same));
+      if (lane == lead) base = atomicAdd(&s.at[wave][e], (int)__builtin_popcountll(same));
       row = __shfl(base, lead) + (int)__builtin_popcountll(same & ((1ull << lane) - 1));
       if (a.src) a.src[row] = slot;
     }
     if (slot < a.n) a.rows[slot] = row;
+  }
+}
+
+__global__ __launch_bounds__(kPlaceThreads) void k_place(DispatchArgs a) {
+  __shared__ PlaceShared s;
+  place(a, blockIdx.x, s);
+}
+
+// The experts' order and the quantized rows of x, side by side in one launch.
+template <int DT>
+__global__ __launch_bounds__(kPlaceThreads) void k_prepare(DispatchArgs a, int chunks, const void* x, int rows, int k, uint8_t* q,
+                                                           float* scales) {
+  __shared__ PlaceShared s;
+  if ((int)blockIdx.x < chunks) return place(a, blockIdx.x, s);
+  // 64 blocks, those of neighbouring rows first
+  const uint32_t at = (blockIdx.x - chunks) * (kPlaceThreads / 16) + (threadIdx.x >> 4);
+  const int kb = (int)(at / (uint32_t)rows), row = (int)(at % (uint32_t)rows);
+  if (kb * kQBlock < k) quantize_block<DT>(x, rows, k, q, scales, row, kb);
+}
+
+// A small batch's order and its rows in one launch: every token's workgroup
+// counts the slots before its own by itself, one ballot for 64 ids and a slot.
+// 64 tokens of 8 x 7168 f16: 9.6 us in two launches -> 4.9.
+constexpr int kMaxSmall = 4096;
+
+template <typename V>
+__global__ __launch_bounds__(256) void k_dispatch_small(DispatchArgs a, int topk, const V* x, V* xs, int len) {
+  __shared__ int ids[kMaxSmall];
+  __shared__ int part[4][64];
+  __shared__ int h[kMaxRouteExperts];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x;
+  const int at0 = blockIdx.y * 256 + tid;
+  V first{};
+  if (at0 < len) first = x[(size_t)t * len + at0];  // on its way while the rows are found
+  for (int i = tid; i < a.n; i += 256) ids[i] = expert_of(a, i);
+  const bool counts = t == 0 && blockIdx.y == 0;
+  if (counts)
+    for (int e = tid; e < a.experts; e += 256) h[e] = 0;
+  __syncthreads();
+  for (int s = 0; s < topk; s++) {
+    const int at = t * topk + s, e = ids[at];
+    int before = 0;
+    for (int i = wave * 64; i < a.n; i += 256) {
+      const int o = i + lane, v = o < a.n ? ids[o] : -1;
+      before += (int)__builtin_popcountll(__ballot(v >= 0 && (v < e || (v == e && o < at))));
+    }
+    if (lane == 0) part[wave][s] = before;
+  }
+  if (counts)
+    for (int i = tid; i < a.n; i += 256)
+      if (ids[i] >= 0) atomicAdd(&h[ids[i]], 1);
+  __syncthreads();
+  if (counts)
+    for (int e = tid; e < a.experts; e += 256) a.counts[e] = h[e];
+  if (tid < topk) {
+    const int row = ids[t * topk + tid] < 0 ? -1 : part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
+    part[0][tid] = row;
+    if (blockIdx.y == 0) a.rows[t * topk + tid] = row;
+  }
+  __syncthreads();
+  for (int i = at0; i < len; i += gridDim.y * 256) {
+    const V v = i == at0 ? first : x[(size_t)t * len + i];
+    for (int s = 0; s < topk; s++) {
+      const int r = part[0][s];
+      if (r >= 0) xs[(size_t)r * len + i] = v;
+    }
   }
 }
 
@@ -284,7 +413,8 @@ __global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
     for (int u = 0; u < N; u++) sum[u] = 0.0f;
   }
   for (int s = 0; s < a.topk; s++) {
-    const int r = a.rows[(size_t)t * a.topk + s];
+    const size_t at = (size_t)t * a.topk + s;
+    const int r = a.rows ? a.rows[at] : (unsigned)a.ids[at] < (unsigned)a.experts ? (int)at : -1;
     if (r < 0) continue;
     const float w = a.weights[(size_t)t * a.topk + s];
     float y[N];
@@ -326,24 +456,53 @@ hipError_t launch_route(int dtype, const RouteArgs& a, hipStream_t st) {
   return hipErrorInvalidValue;
 }
 
-static int chunks_of(int n) { return (n + kChunk - 1) / kChunk; }
-size_t dispatch_ws_bytes(int n, int experts) { return chunks_of(n) > 1 ? (size_t)chunks_of(n) * experts * 4 : 0; }
+static int chunks_of(int n) { return n > 0 ? (n + kChunk - 1) / kChunk : 1; }
+size_t dispatch_ws_bytes(int n, int experts) { return n > kMaxCounted ? (size_t)chunks_of(n) * experts * 4 : 0; }
 
-hipError_t launch_dispatch(const DispatchArgs& a, hipStream_t st) {
-  const int chunks = chunks_of(a.n);
-  if (chunks > 1) hipLaunchKernelGGL(k_count, dim3(chunks), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(k_place, dim3(chunks > 0 ? chunks : 1), dim3(256), 0, st, a, chunks > 0 ? chunks : 1);
+static hipError_t count_many(DispatchArgs& a, hipStream_t st) {
+  if (a.n <= kMaxCounted) {
+    a.hist = nullptr;
+    return hipSuccess;
+  }
+  hipLaunchKernelGGL(k_count, dim3(chunks_of(a.n)), dim3(kPlaceThreads), 0, st, a);
   return hipGetLastError();
 }
 
-hipError_t launch_gather(const void* x, const int32_t* rows, void* xs, int tokens, int topk, size_t row_bytes,
-                         hipStream_t st) {
+hipError_t launch_dispatch(const DispatchArgs& a0, hipStream_t st) {
+  DispatchArgs a = a0;
+  if (hipError_t e = count_many(a, st)) return e;
+  hipLaunchKernelGGL(k_place, dim3(chunks_of(a.n)), dim3(kPlaceThreads), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_prepare(const DispatchArgs& a0, int dtype, const void* x, int rows, int k, uint8_t* q, float* scales,
+                          hipStream_t st) {
+  DispatchArgs a = a0;
+  if (hipError_t e = count_many(a, st)) return e;
+  const int chunks = chunks_of(a.n);
+  const long groups = (long)rows * ((k + kQBlock - 1) / kQBlock), per = kPlaceThreads / 16;
+  if (groups > 0x7fffffffL) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(chunks + (groups + per - 1) / per));
+  if (dtype == MX_DTYPE_F16) hipLaunchKernelGGL((k_prepare<MX_DTYPE_F16>), grid, dim3(kPlaceThreads), 0, st, a, chunks, x, rows, k, q, scales);
+  else hipLaunchKernelGGL((k_prepare<MX_DTYPE_BF16>), grid, dim3(kPlaceThreads), 0, st, a, chunks, x, rows, k, q, scales);
+  return hipGetLastError();
+}
+
+hipError_t launch_dispatch_rows(const DispatchArgs& a, int topk, const void* x, void* xs, size_t row_bytes, hipStream_t st) {
+  const int tokens = a.n / topk;
+  const bool small = a.n <= kMaxSmall && (long)a.n * topk <= 8 * kMaxSmall;
+  if (!small)
+    if (hipError_t e = launch_dispatch(a, st)) return e;
   const uintptr_t p = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xs);
   auto go = [&](auto v) {
     using V = decltype(v);
     const int len = (int)(row_bytes / sizeof(V));
-    hipLaunchKernelGGL((k_gather<V>), dim3(tokens, (len + 255) / 256), dim3(256), 0, st, static_cast<const V*>(x), rows,
-                       static_cast<V*>(xs), topk, len);
+    const V* from = static_cast<const V*>(x);
+    V* to = static_cast<V*>(xs);
+    // few tokens: their rows are split over workgroups
+    const int parts = tokens >= 256 ? 1 : (len + 255) / 256;
+    if (small) hipLaunchKernelGGL((k_dispatch_small<V>), dim3(tokens, parts), dim3(256), 0, st, a, topk, from, to, len);
+    else hipLaunchKernelGGL((k_gather<V>), dim3(tokens, (len + 255) / 256), dim3(256), 0, st, from, a.rows, to, topk, len);
   };
   if (row_bytes % 16 == 0 && p % 16 == 0) go(v4i{});
   else if (row_bytes % 4 == 0 && p % 4 == 0) go(uint32_t{});

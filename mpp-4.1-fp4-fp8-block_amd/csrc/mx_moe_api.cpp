@@ -48,6 +48,45 @@ int check_experts(mx_ctx* c, int experts) {
   return MX_OK;
 }
 
+// mx_moe_block_forward of one token: its slots need no order, and its few rows are
+// quantized where they are used.
+int block_experts_of_one(mx_ctx* c, int H, int I, int E, int topk, const void* x, int dtype, const int32_t* ids,
+                         const float* weights, const mx_mlp_weights* w, const void* add, void* out) {
+  const size_t mid = ((size_t)topk * I * 4 + 255) / 256 * 256;
+  void* p = nullptr;
+  if (int rc = mx_ctx_workspace(c, mid + (size_t)topk * H * 4, &p)) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(p);
+  hipStream_t st = mx_ctx_stream(c);
+  mx::BlockGemmArgs g{};
+  g.m = topk;
+  g.ids = ids;
+  g.experts = E;
+  g.splits = 1;
+  g.raw = x;
+  g.w0 = static_cast<const uint8_t*>(w->gate.data);
+  g.w1 = static_cast<const uint8_t*>(w->up.data);
+  g.s0 = static_cast<const float*>(w->gate.scales);
+  g.s1 = static_cast<const float*>(w->up.scales);
+  g.w_stride = (size_t)I * H;
+  g.s_stride = (size_t)blocks(I) * blocks(H);
+  g.c = ws;
+  g.n = I;
+  g.k = H;
+  MX_RUN(c, mx::launch_block_direct(dtype, g, st));
+  g.raw = ws;
+  g.row_per_slot = 1;
+  g.w0 = static_cast<const uint8_t*>(w->down.data);
+  g.w1 = nullptr;
+  g.s0 = static_cast<const float*>(w->down.scales);
+  g.c = ws + mid;
+  g.n = H;
+  g.k = I;
+  MX_RUN(c, mx::launch_block_direct(MX_DTYPE_F32, g, st));
+  const mx::CombineArgs b{ws + mid, nullptr, weights, add, out, 1, topk, H, ids, E};
+  MX_RUN(c, mx::launch_combine(MX_DTYPE_F32, dtype, b, st));
+  return MX_OK;
+}
+
 // One pass of mx_moe_block_forward over T >= 1 tokens.
 int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x, int dtype, const int32_t* ids,
                   const float* weights, const mx_mlp_weights* w, const void* add, void* out) {
@@ -72,8 +111,7 @@ int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x
   mx::DispatchArgs d{ids, n, E, reinterpret_cast<int32_t*>(ws + o_counts), reinterpret_cast<int32_t*>(ws + o_rows),
                      reinterpret_cast<int32_t*>(ws + o_src), reinterpret_cast<mx::RowTile*>(ws + o_tiles),
                      reinterpret_cast<int32_t*>(ws + o_nt), tile_rows, reinterpret_cast<int32_t*>(ws + o_hist)};
-  MX_RUN(c, mx::launch_dispatch(d, st));
-  MX_RUN(c, mx::launch_block_quantize(dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), st));
+  MX_RUN(c, mx::launch_prepare(d, dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), st));
   mx::BlockGemmArgs g{};
   g.a = ws + o_xq;
   g.a_s = reinterpret_cast<float*>(ws + o_xs);
@@ -110,7 +148,7 @@ int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x
   g.k = I;
   g.src = nullptr;
   MX_RUN(c, mx::launch_block_gemm(y_dtype, g, st));
-  const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H};
+  const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H, nullptr, 0};
   MX_RUN(c, mx::launch_combine(y_dtype, dtype, b, st));
   return MX_OK;
 }
@@ -179,9 +217,8 @@ int mx_moe_dispatch(mx_ctx* c, int tokens, int topk, int experts, const int32_t*
   a.counts = counts;
   a.rows = rows;
   a.hist = static_cast<int32_t*>(ws);
-  MX_RUN(c, mx::launch_dispatch(a, mx_ctx_stream(c)));
-  if (x && tokens)
-    MX_RUN(c, mx::launch_gather(x, rows, xs, tokens, topk, (size_t)hidden * size_of(dtype), mx_ctx_stream(c)));
+  if (x && tokens) MX_RUN(c, mx::launch_dispatch_rows(a, topk, x, xs, (size_t)hidden * size_of(dtype), mx_ctx_stream(c)));
+  else MX_RUN(c, mx::launch_dispatch(a, mx_ctx_stream(c)));
   return MX_OK;
 }
 
@@ -196,7 +233,7 @@ int mx_moe_combine(mx_ctx* c, int tokens, int topk, int hidden, const void* y, i
   if (!is_aligned(y, size_of(y_dtype)) || !is_aligned(add, size_of(out_dtype)) || !is_aligned(out, size_of(out_dtype)) ||
       !is_aligned(rows, 4) || !is_aligned(weights, 4))
     return fail(c, MX_EINVAL, "combine buffers must be aligned to their elements.");
-  const mx::CombineArgs a{y, rows, weights, add, out, tokens, topk, hidden};
+  const mx::CombineArgs a{y, rows, weights, add, out, tokens, topk, hidden, nullptr, 0};
   MX_RUN(c, mx::launch_combine(y_dtype, out_dtype, a, mx_ctx_stream(c)));
   return MX_OK;
 }
@@ -264,6 +301,8 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
   if (!x || !ids || !weights || !out) return fail(c, MX_EINVAL, "MoE buffers must not be null.");
   if (!is_aligned(x, 16) || !is_aligned(out, 16) || !is_aligned(add, 16) || !is_aligned(ids, 4) || !is_aligned(weights, 4))
     return fail(c, MX_EINVAL, "MoE rows must be 16-byte aligned, ids and weights 4-byte.");
+  if (T == 1 && H <= mx::kMaxDirect && I <= mx::kMaxDirect)
+    return block_experts_of_one(c, H, I, E, topk, x, dtype, ids, weights, w, add, out);
   // The picked rows of x are addressed by 31 bits: larger batches in parts.
   const int most = (int)(0x7fff0000u / (uint32_t)H);
   for (int t = 0; t < T; t += most) {
