@@ -1070,8 +1070,8 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
   size_t off = 0;
   auto take = [&](size_t bytes) { size_t o = off; off = align_up(off + bytes, 256); return o; };
   const size_t bh = (H + mx::kQBlock - 1) / mx::kQBlock, bi = (I + mx::kQBlock - 1) / mx::kQBlock;
-  const int gu_rows = mx::block_tile_rows(T, 1, I, MX_DTYPE_F32, true);
-  const bool few = gu_rows == 16;  // the middle comes in f32; else in its codes
+  const int gu_rows = mx::block_tile_rows(T, 1, I, H, MX_DTYPE_F16, true);
+  const bool few = mx::block_streams(gu_rows);  // the middle comes in f32; else in its codes
   const size_t o_xq = take((size_t)T * H), o_xs = take(T * bh * 4), o_mid = take(few ? (size_t)T * I * 4 : 0),
                o_mq = take((size_t)T * I), o_ms = take(T * bi * 4);
   if (int rc = ensure_ws(c, off)) return rc;
@@ -1086,7 +1086,7 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
   gu.c = few ? static_cast<void*>(mid) : mq; gu.c_s = ms;
   gu.w0 = static_cast<const uint8_t*>(w->gate.data); gu.s0 = static_cast<const float*>(w->gate.scales);
   gu.w1 = static_cast<const uint8_t*>(w->up.data); gu.s1 = static_cast<const float*>(w->up.scales);
-  dn.a = mq; dn.a_s = ms; dn.a_rows = dn.m = T; dn.n = H; dn.k = I; dn.c = out; dn.tile_rows = mx::block_tile_rows(T, 1, H, MX_DTYPE_F16, false);
+  dn.a = mq; dn.a_s = ms; dn.a_rows = dn.m = T; dn.n = H; dn.k = I; dn.c = out; dn.tile_rows = mx::block_tile_rows(T, 1, H, I, MX_DTYPE_F16, false);
   dn.w0 = static_cast<const uint8_t*>(w->down.data); dn.s0 = static_cast<const float*>(w->down.scales);
   steps.push_back({"block_quantize_x", [=] { return mx::launch_block_quantize(MX_DTYPE_F16, x, T, H, xq, xs, st); }});
   steps.push_back({mx_fmt_mlp_kernel_name(MX_WFMT_FP8_BLOCK, cfg, 1), [=] { return mx::launch_block_gemm(MX_DTYPE_F32, gu, st); }});
@@ -1220,7 +1220,8 @@ const char* mx_fmt_mlp_kernel_name(int wfmt, const mx_mlp_config* cfg, int index
   static const char* block3[] = {"block_quantize_x", "block_gemm_gate_up_swiglu_quantize", "block_gemm_down"};
   if (index < 0 || !cfg || wfmt < MX_WFMT_FP8_E4M3 || wfmt > MX_WFMT_FP8_BLOCK) return nullptr;
   if (wfmt == MX_WFMT_FP8_BLOCK) {
-    if (mx::block_tile_rows(cfg->tokens, 1, cfg->intermediate, MX_DTYPE_F32, true) == 16) return index < 4 ? block[index] : nullptr;
+    if (mx::block_streams(mx::block_tile_rows(cfg->tokens, 1, cfg->intermediate, cfg->hidden, MX_DTYPE_F16, true)))
+      return index < 4 ? block[index] : nullptr;
     return index < 3 ? block3[index] : nullptr;
   }
   if (wfmt == MX_WFMT_W8A8) return index < 4 ? w8a8[index] : nullptr;

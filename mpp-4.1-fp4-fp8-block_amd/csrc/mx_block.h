@@ -97,12 +97,13 @@ struct BlockGemmArgs {
   const int32_t* ids;                // [m] the slots' experts
   int experts;
 };
-// Activation rows of a tile for `rows` rows in `groups` matrices of n rows: 16
-// (weights streamed), 64 or 256.
-int block_tile_rows(long rows, int groups, int n, int c_dtype, bool swiglu);
+// Activation rows of a tile for `rows` rows in `groups` matrices [n][k]: 16 or 32
+// (weights streamed), 64, 128 (f32 results) or 256.
+int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swiglu);
 int block_splits(int m, int n, int k, int tile_rows);
-// The product by tiles of g.tile_rows rows.  SwiGLU: tiles of 16 rows write f32
-// [m][n] to c, larger ones E4M3 codes to c and their scales to c_s.
+// The product by tiles of g.tile_rows rows.  SwiGLU: streamed tiles write
+// f32 [m][n] to c, larger ones E4M3 codes to c and their scales to c_s.
+inline bool block_streams(int tile_rows) { return tile_rows <= 32; }
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st);
 hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st);  // mx_block_stream.hip
 // One token, k <= kMaxDirect: gate/up products of an f16 or bf16 row or the down

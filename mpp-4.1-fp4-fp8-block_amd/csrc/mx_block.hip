@@ -63,17 +63,39 @@ hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_
   return hipGetLastError();
 }
 
-int block_tile_rows(long rows, int groups, int n, int c_dtype, bool swiglu) {
+// Streamed tiles keep the weights' way from HBM busy and cost a fetch of the
+// weights for each; the others cost rounds of the CUs by a stage's time, in us,
+// as measured (a stage: one 128-block of K):
+//   64 rows    0.57 a stage up to 256 tiles, 0.9 for two on a CU; in f16 (f32
+//              results, SwiGLU) 0.85 and 1.2
+//   128 rows   1.6, f32 results only
+//   256 rows   1.05
+// 1000 rows of 4096 -> 4096: 30 us with 64 rows and 38 with 256; 4096 rows 110 and
+// 80.  16 experts with 32 rows each run on 64-row tiles, which sum SwiGLU's products
+// in f16, from 48 rows on on 256-row tiles, which read each expert's weights once.
+int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swiglu) {
   const long each = (rows + groups - 1) / groups;
+  if (groups > 1) {  // experts differ in rows: room for more than the mean
+    if (each <= 4) return 16;
+    if (each <= 20) return 32;
+    if (swiglu) return each <= 48 ? 64 : 256;
+  }
   if (each <= 16) return 16;
-  // f32 results keep more bits than the FP8 matrix cores' sums hold
-  if (!swiglu && c_dtype == MX_DTYPE_F32) return 64;
-  const long tiles = groups * ((each + 255) / 256) * ((n + 255) / 256) * (swiglu ? 2 : 1);
-  return each >= 160 && tiles >= 128 ? 256 : 64;
+  // two fetches of small weights come from the cache
+  if (each <= 32) return ((swiglu ? n * 2L : n) + 31) / 32 <= 192 ? 16 : 32;
+  const bool f16_sums = swiglu || c_dtype == MX_DTYPE_F32;
+  const double kb = (k + kQBlock - 1) / kQBlock;
+  auto rounds = [](long tiles, long at_once) { return (double)((tiles + at_once - 1) / at_once); };
+  auto tiles = [&](long r, long c) { return groups * ((each + r - 1) / r) * ((n + c - 1) / c); };
+  const long t64 = tiles(64, 128);
+  const double us64 = t64 <= 256 ? kb * (f16_sums ? 0.85 : 0.57) + 5
+                                 : rounds(t64, swiglu ? 256 : 512) * (kb * (f16_sums ? 1.2 : 0.9) + 5);
+  if (!swiglu && c_dtype == MX_DTYPE_F32) return rounds(tiles(128, 256), 256) * (kb * 1.6 + 6) < us64 ? 128 : 64;
+  return rounds(tiles(256, swiglu ? 128 : 256), 256) * (kb * 1.05 + 6) < us64 ? 256 : 64;
 }
 
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
-  return g.tile_rows == 16 ? launch_block_stream(c_dtype, g, st) : launch_block_tile(c_dtype, g, st);
+  return block_streams(g.tile_rows) ? launch_block_stream(c_dtype, g, st) : launch_block_tile(c_dtype, g, st);
 }
 
 }  // namespace mx

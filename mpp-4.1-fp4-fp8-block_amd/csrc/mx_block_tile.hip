@@ -348,13 +348,17 @@ hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
 
 template <int DT>
 hipError_t store_tiles(const BlockGemmArgs& g, hipStream_t st) {
-  if constexpr (DT != MX_DTYPE_F32) {
+  // f32 results keep more bits than the FP8 matrix cores' sums hold
+  constexpr bool WIDE = DT == MX_DTYPE_F32;
+  if constexpr (WIDE) {
+    if (g.tile_rows == 128) return launch_one<DT, false, 256, 128, 4, 2, 3, true>(g, st);
+  } else {
     if (g.tile_rows == 256) return launch_one<DT, false, 256, 256, 4, 2, 2, false>(g, st);
   }
-  if (g.splits == 1) return launch_one<DT, false, 128, 64, 4, 1, 3, true>(g, st);
+  if (g.splits == 1) return launch_one<DT, false, 128, 64, 4, 1, 3, WIDE>(g, st);
   BlockGemmArgs p = g;
   p.c = g.part;
-  if (hipError_t e = launch_one<MX_DTYPE_F32, false, 128, 64, 4, 1, 3, true>(p, st)) return e;
+  if (hipError_t e = launch_one<MX_DTYPE_F32, false, 128, 64, 4, 1, 3, WIDE>(p, st)) return e;
   const size_t len = (size_t)g.m * g.n;
   const float* part = static_cast<const float*>(g.part);
   if (len % 8 == 0) hipLaunchKernelGGL((k_block_join<DT, 8>), dim3((unsigned)((len / 8 + 255) / 256)), dim3(256), 0, st, part, len, g.splits, g.c);
@@ -364,14 +368,16 @@ hipError_t store_tiles(const BlockGemmArgs& g, hipStream_t st) {
 
 }  // namespace
 
-// Parts of K for a dense product by 64-row tiles: about two workgroups a CU,
-// each with four blocks at least.
+// Parts of K for a dense product by 64-row tiles that would leave half of the CUs
+// idle: about a workgroup a CU, each with four blocks at least.  The parts' sum
+// costs a launch (3.5 us): 46 rows of 3968 -> 1221 17.5 us in one part and 10.4 in
+// seven, 300 rows of 4096 -> 4096 (160 tiles) 19.9 in one and 19.6 in two.
 int block_splits(int m, int n, int k, int tile_rows) {
   if (tile_rows != 64) return 1;
   const long tiles = (long)((m + 63) / 64) * ((n + 127) / 128);
-  const int kb = (k + kQBlock - 1) / kQBlock;
-  const long s = 512 / tiles;
-  return s <= 1 ? 1 : s > kb / 4 ? (kb / 4 > 1 ? kb / 4 : 1) : (int)s;
+  if (tiles >= 128) return 1;
+  const long s = 256 / tiles, most = (k + kQBlock - 1) / kQBlock / 4;
+  return (int)(s < most ? s : most > 1 ? most : 1);
 }
 
 hipError_t launch_block_tile(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {

@@ -94,11 +94,11 @@ int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x
   size_t off = 0;
   auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
   // one tile height for both products, so that they share the list of tiles
-  const int used = n < E ? n : E, tile_rows = mx::block_tile_rows(n, used, I, dtype, true), max_tiles = used + n / tile_rows;
+  const int used = n < E ? n : E, tile_rows = mx::block_tile_rows(n, used, I, H, dtype, true), max_tiles = used + n / tile_rows;
   // Few rows keep the middle and the experts' rows in f32; more of them the
   // middle in its codes alone and the experts' rows in the rows' type, one
   // rounding more for half the bytes.
-  const bool few = tile_rows == 16;
+  const bool few = mx::block_streams(tile_rows);
   const int y_dtype = few ? MX_DTYPE_F32 : dtype;
   const size_t o_xq = take((size_t)T * H), o_xs = take((size_t)T * blocks(H) * 4), o_rows = take((size_t)n * 4),
                o_src = take((size_t)n * 4), o_counts = take((size_t)E * 4), o_tiles = take((size_t)max_tiles * sizeof(mx::RowTile)),
@@ -270,7 +270,7 @@ int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const ui
   g.m = m;
   g.n = n;
   g.k = k;
-  g.tile_rows = mx::block_tile_rows(m, 1, n, c_dtype, false);
+  g.tile_rows = mx::block_tile_rows(m, 1, n, k, c_dtype, false);
   g.splits = mx::block_splits(m, n, k, g.tile_rows);
   if (g.splits > 1)
     if (int rc = mx_ctx_workspace(c, (size_t)g.splits * m * n * 4, &g.part)) return rc;
