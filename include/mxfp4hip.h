@@ -281,7 +281,7 @@ int mx_moe_benchmark(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, const
 /* No counterpart in the reference.  From gate logits to mx_moe_forward's rows
  * and counts, and from its rows back to tokens.  All of it stays on the device
  * in stream order; tokens = 0 is allowed and does nothing else than to clear
- * the counts. */
+ * the counts.  topk <= 64 and tokens * topk < 2^26. */
 enum { MX_ROUTE_SOFTMAX = 0, MX_ROUTE_SIGMOID = 1 };
 typedef struct {
   uint32_t tokens, experts, topk;   /* experts <= 512, topk <= 64 */
@@ -327,12 +327,14 @@ int mx_moe_combine(mx_ctx* ctx, int tokens, int topk, int hidden, const void* y,
  * (f32, f16, bf16) -> q [rows][k], scales [ceil(k/128)][rows].  scale =
  * amax * (1/448 in f32), at least 2^-126, 1 where all 128 are zero; code =
  * E4M3(x / scale), an f32 division, to nearest even.  128 values with a NaN or an infinity among them come out
- * as NaN.  k % 16 == 0; rows = 0 is allowed. */
+ * as NaN.  k % 16 == 0, k <= 65536; rows = 0 is allowed. */
 int mx_block_quantize(mx_ctx* ctx, const void* src, int src_dtype, int rows, int k, uint8_t* q, float* scales);
 /* C[m][n] = sum over 128-blocks kb of a_scales[kb][m] * b_scales[n/128][kb] *
  * sum_{k in kb} A[m][k] * B[n][k], with A as mx_block_quantize and B [n][k] as
  * mx_fmt_quantize(MX_WFMT_FP8_BLOCK) writes them; f32 sums, C f32, f16 or
- * bf16.  Any n >= 1, k % 16 == 0, k <= 65536; m = 0 is allowed. */
+ * bf16.  f16 and bf16 results of more than 32 rows come from the FP8 matrix cores,
+ * whose sums hold about 1e-5 of their value; f32 results and few rows from f16
+ * products with f32 sums.  Any n >= 1, k % 16 == 0, k <= 65536; m = 0 is allowed. */
 int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const uint8_t* b,
                     const float* b_scales, void* c, int c_dtype, int m, int n, int k);
 /* The MLP of each token's experts with block-scaled FP8 weights, from token

@@ -76,7 +76,7 @@ hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_
 int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swiglu) {
   const long each = (rows + groups - 1) / groups;
   if (groups > 1) {  // experts differ in rows: room for more than the mean
-    if (each <= 4) return 16;
+    if (each <= 6) return 16;
     if (each <= 20) return 32;
     if (swiglu) return each <= 48 ? 64 : 256;
   }

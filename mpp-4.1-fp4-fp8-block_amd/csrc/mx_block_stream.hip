@@ -1,5 +1,12 @@
 // mx_block_stream.hip - products of block-scaled FP8 weights with at most 32
 // activation rows a tile: the weights stream from HBM to registers once.
+//
+// Bound: HBM.  A wave takes every W-th block of K of its workgroup's weight rows,
+// straight to registers, in whole 128-byte lines (8 rows a load, the halves then
+// exchanged between lanes); no wave waits for another before the final sum.  The
+// products are f16 MFMAs of the widened codes, whose sums are f32: the matrix cores
+// have time for that while the weights come in.  One token's 352 MB through 8 of 64
+// experts: 43 us gate/up (5.5 TB/s) and 23 us down (5.1), where a copy reaches 4.9.
 #include "mx_block.h"
 #include "mx_block_device.h"
 
@@ -200,15 +207,21 @@ hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
   return hipGetLastError();
 }
 
-// 32 weight rows a workgroup, whose 4 waves each have three blocks of K under way:
-// 352 MB of eight experts at 5.5 TB/s.  Where that leaves CUs idle, 16 rows (with
-// SwiGLU 32) and 8 waves: one row of 7552 -> 2560 12.9 -> 7.9 us, of 4096 -> 4096
-// 8.7 -> 7.1, but of 4096 -> 14336 14.8 -> 16.4.
+// 32 weight rows a workgroup of 4 waves.  Blocks under way in a wave: where K is
+// short, one, and more waves on a CU (32 experts' 1408 -> 4096, 10 rows each: 37 us,
+// 39 with two and 45 with three); past 4096 two (one token's gate and up products
+// of 7168: 43, 47 with one).  One token, whose activations take no registers: three.
+// Where the tiles leave CUs idle, 16 rows (with SwiGLU 32) and 8 waves: one row of
+// 7552 -> 2560 12.9 -> 7.9 us, of 4096 -> 4096 8.7 -> 7.1, but of 4096 -> 14336 14.8
+// -> 16.4.
 template <int DT, bool DUAL, int TT, int XT>
 hipError_t launch_shape(const BlockGemmArgs& g, hipStream_t st) {
   const long tiles = (long)(XT >= 0 ? g.m : g.tiles ? g.max_tiles : (g.m + 16 * TT - 1) / (16 * TT)) * ((g.n + 31) / 32);
-  if (TT == 1 && tiles * (DUAL ? 2 : 1) < 256) return launch_one<DT, DUAL, DUAL ? 2 : 1, 8, 2, TT, XT>(g, st);
-  return launch_one<DT, DUAL, 2, 4, 3, TT, XT>(g, st);
+  if constexpr (TT == 1) {
+    if (tiles * (DUAL ? 2 : 1) < 256) return launch_one<DT, DUAL, DUAL ? 2 : 1, 8, 2, TT, XT>(g, st);
+  }
+  if constexpr (XT >= 0) return launch_one<DT, DUAL, 2, 4, 3, TT, XT>(g, st);
+  else return g.k <= 32 * kQBlock ? launch_one<DT, DUAL, 2, 4, 1, TT, XT>(g, st) : launch_one<DT, DUAL, 2, 4, 2, TT, XT>(g, st);
 }
 
 template <int TT>

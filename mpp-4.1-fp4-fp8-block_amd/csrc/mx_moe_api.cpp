@@ -35,10 +35,10 @@ bool is_float(int dtype) { return dtype == MX_DTYPE_F32 || dtype == MX_DTYPE_F16
 size_t size_of(int dtype) { return dtype == MX_DTYPE_F32 ? 4 : 2; }
 int blocks(int n) { return (n + mx::kQBlock - 1) / mx::kQBlock; }
 
-// slots of a batch: tokens and pairs have to be counted in 31 bits
+// slots of a batch
 int check_slots(mx_ctx* c, int tokens, int topk) {
   if (tokens < 0 || topk < 1 || topk > 64) return fail(c, MX_EINVAL, "MoE needs tokens >= 0 and topk in 1..64.");
-  if ((long long)tokens * topk > 0x3fffffff) return fail(c, MX_EINVAL, "MoE tokens x topk must be below 2^30.");
+  if ((long long)tokens * topk >= 1 << 26) return fail(c, MX_EINVAL, "MoE tokens x topk must be below 2^26.");
   return MX_OK;
 }
 
@@ -241,6 +241,7 @@ int mx_moe_combine(mx_ctx* c, int tokens, int topk, int hidden, const void* y, i
 int mx_block_quantize(mx_ctx* c, const void* src, int src_dtype, int rows, int k, uint8_t* q, float* scales) {
   if (!c) return MX_EINVAL;
   if (rows < 0 || k <= 0 || k % 16) return fail(c, MX_EINVAL, "block quantize needs rows >= 0 and k a positive multiple of 16.");
+  if (k > mx::kMaxBlocks * mx::kQBlock) return fail(c, MX_EINVAL, "block quantize k is at most %d.", mx::kMaxBlocks * mx::kQBlock);
   if (!is_float(src_dtype)) return fail(c, MX_EINVAL, "block quantize source must be f32, f16 or bf16.");
   if (rows == 0) return MX_OK;
   if (!src || !q || !scales || !is_aligned(src, 16) || !is_aligned(q, 16) || !is_aligned(scales, 4))
