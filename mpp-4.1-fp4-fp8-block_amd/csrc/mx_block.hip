@@ -91,7 +91,9 @@ int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swigl
   const double us64 = t64 <= 256 ? kb * (f16_sums ? 0.85 : 0.57) + 5
                                  : rounds(t64, swiglu ? 256 : 512) * (kb * (f16_sums ? 1.2 : 0.9) + 5);
   if (!swiglu && c_dtype == MX_DTYPE_F32) return rounds(tiles(128, 256), 256) * (kb * 1.6 + 6) < us64 ? 128 : 64;
-  return rounds(tiles(256, swiglu ? 128 : 256), 256) * (kb * 1.05 + 6) < us64 ? 256 : 64;
+  // (after others, a last round for at most half of the CUs takes about half of one)
+  const long t256 = tiles(256, swiglu ? 128 : 256), last = t256 % 256;
+  return (t256 / 256 + (last == 0 ? 0 : last <= 128 && t256 > 256 ? 0.55 : 1)) * (kb * 1.05 + 6) < us64 ? 256 : 64;
 }
 
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {

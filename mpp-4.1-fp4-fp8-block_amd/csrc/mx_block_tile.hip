@@ -39,6 +39,7 @@
 namespace mx {
 namespace {
 
+constexpr int kCUs = 256;           // of an MI355X, 32 in each of 8 XCDs
 constexpr int kPast = 0x7fffff00;  // past every resource's range
 constexpr int lgkm0_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4); }
 __device__ __forceinline__ void dma16(v4i rsrc, void* lds, int lane_offset, int offset) {
@@ -76,8 +77,17 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   const int NT = (g.n + TN / ND - 1) / (TN / ND), MT = g.tiles ? *g.n_tiles : (g.m + TM - 1) / TM;
   // An XCD takes a run of neighbouring tiles, 8 weight tiles by all row tiles: its
   // 32 CUs then work on about 8 weight and 4 row tiles and fetch each once.
-  const int total = MT * NT * g.splits, per = (total + 7) / 8, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || at >= total) return;
+  const int total = MT * NT * g.splits, per = (total + 7) / 8;
+  int mine = blockIdx.x >> 3, half = 0;  // of the XCD's run
+  // A last round for at most half of the CUs: its tiles go to two workgroups each.
+  const int rest = TM == 256 ? per % (kCUs / 8) : 0;
+  const bool halves = rest && rest <= kCUs / 16 && mine >= per - rest;
+  if (halves) {
+    half = (mine - (per - rest)) & 1;
+    mine = per - rest + (mine - (per - rest)) / 2;
+  }
+  const int at = (blockIdx.x & 7) * per + mine;
+  if (mine >= per || at >= total) return;
   const int sp = at / (MT * NT), tile = at % (MT * NT);
   const int grp = tile / (8 * MT), in = tile % (8 * MT), gw = min(8, NT - grp * 8);
   const int rt = in / gw, n0 = (grp * 8 + in % gw) * (TN / ND);
@@ -87,6 +97,11 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
     row0 = t.row0;
     rows = t.rows;
     expert = t.expert;
+  }
+  if (halves) {
+    row0 += half * (TM / 2);
+    rows = min(TM / 2, rows - half * (TM / 2));
+    if (rows <= 0) return;
   }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
@@ -184,9 +199,9 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   // every WM-th run of 16 activation rows, so that the waves of a tile with few
   // rows are left with equally many.
   auto arow = [&](int j) { return (j * WM + wm) * 16; };
-  int mine = lane;
-  asm volatile("" : "+v"(mine));  // (a value of this body: the bodies' common parts are not worked out before them)
-  const int r16 = mine & 15, kq = mine >> 4;
+  int here = lane;
+  asm volatile("" : "+v"(here));  // (a value of this body: the bodies' common parts are not worked out before them)
+  const int r16 = here & 15, kq = here >> 4;
   const int sw = place_key(r16), off0 = r16 * 128 + (((2 * kq) ^ sw) << 4), off1 = r16 * 128 + (((2 * kq + 1) ^ sw) << 4);
   auto wrow = [&](int i) { return DUAL ? (i < NI / 2 ? wn * (CN / 2) + i * 16 : TN / 2 + wn * (CN / 2) + (i - NI / 2) * 16) : wn * CN + i * 16; };
   auto frag = [&](const uint8_t* s, int row) __attribute__((always_inline)) -> v8i {
@@ -371,9 +386,9 @@ template <int DT, bool DUAL, int TN, int TM, int WN, int WM, int NS, bool WIDE>
 hipError_t launch_one(const BlockGemmArgs& g, hipStream_t st) {
   const int nt = (g.n + TN / (DUAL ? 2 : 1) - 1) / (TN / (DUAL ? 2 : 1));
   const long tiles = (long)(g.tiles ? g.max_tiles : (g.m + TM - 1) / TM) * nt * g.splits;
-  if (tiles > 0x7ffffff0L) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_block_tile<DT, DUAL, TN, TM, WN, WM, NS, WIDE>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
-                     st, g);
+  if (tiles > 0x7fffff00L) return hipErrorInvalidValue;
+  const unsigned grid = (unsigned)((tiles + 7) / 8 * 8) + (TM == 256 ? kCUs / 2 : 0);  // (room for the halved tiles)
+  hipLaunchKernelGGL((k_block_tile<DT, DUAL, TN, TM, WN, WM, NS, WIDE>), dim3(grid), dim3(64 * WN * WM), 0, st, g);
   return hipGetLastError();
 }
 
