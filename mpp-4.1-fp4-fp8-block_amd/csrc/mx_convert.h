@@ -66,4 +66,32 @@ __device__ __forceinline__ void store_n_from_f32(void* p, size_t i, const float*
   }
 }
 
+// Eight values at any address of their type, or the `left` that there still are (the
+// others: 0, not stored).
+template <int DT>
+__device__ __forceinline__ void load_some_as_f32(const void* p, size_t i, int left, float* v) {
+  constexpr int SIZE = DT == MX_DTYPE_F32 ? 4 : 2;
+  if (left >= 8) {
+    __attribute__((aligned(16))) uint8_t raw[8 * SIZE];
+    __builtin_memcpy(raw, static_cast<const uint8_t*>(p) + i * SIZE, sizeof raw);
+    load_n_as_f32<DT, 8>(raw, 0, v);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 8; u++) v[u] = u < left ? load_as_f32<DT>(p, i + u) : 0.0f;
+}
+template <int DT>
+__device__ __forceinline__ void store_some_from_f32(void* p, size_t i, int left, const float* v) {
+  constexpr int SIZE = DT == MX_DTYPE_F32 ? 4 : 2;
+  if (left >= 8) {
+    __attribute__((aligned(16))) uint8_t raw[8 * SIZE];
+    store_n_from_f32<DT, 8>(raw, 0, v);
+    __builtin_memcpy(static_cast<uint8_t*>(p) + i * SIZE, raw, sizeof raw);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 8; u++)
+    if (u < left) store_from_f32<DT>(p, i + u, v[u]);
+}
+
 }  // namespace mx

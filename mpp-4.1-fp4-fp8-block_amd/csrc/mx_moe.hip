@@ -341,20 +341,42 @@ __global__ __launch_bounds__(kPlaceThreads) void k_prepare(DispatchArgs a, int c
   if (kb * kQBlock < k) quantize_block<DT>(x, rows, k, q, scales, row, kb);
 }
 
+// 16 bytes at any even address, or the `left` that a row still has.
+__device__ __forceinline__ void load16(const uint8_t* p, size_t left, v4i& v) {
+  if (left >= 16) {
+    __builtin_memcpy(&v, p, 16);
+    return;
+  }
+  uint16_t h[8];
+#pragma unroll
+  for (int u = 0; u < 8; u++) h[u] = (size_t)u * 2 < left ? reinterpret_cast<const uint16_t*>(p)[u] : (uint16_t)0;
+  __builtin_memcpy(&v, h, 16);
+}
+__device__ __forceinline__ void store16(uint8_t* p, size_t left, const v4i& v) {
+  if (left >= 16) {
+    __builtin_memcpy(p, &v, 16);
+    return;
+  }
+  uint16_t h[8];
+  __builtin_memcpy(h, &v, 16);
+#pragma unroll
+  for (int u = 0; u < 8; u++)
+    if ((size_t)u * 2 < left) reinterpret_cast<uint16_t*>(p)[u] = h[u];
+}
+
 // A small batch's order and its rows in one launch: every token's workgroup
 // counts the slots before its own by itself, one ballot for 64 ids and a slot.
-// 64 tokens of 8 x 7168 f16: 9.6 us in two launches -> 4.9.
+// 64 tokens of 8 x 7168 f16: 9.6 us in two launches -> 6.1.
 constexpr int kMaxSmall = 4096;
 
-template <typename V>
-__global__ __launch_bounds__(256) void k_dispatch_small(DispatchArgs a, int topk, const V* x, V* xs, int len) {
+__global__ __launch_bounds__(256) void k_dispatch_small(DispatchArgs a, int topk, const uint8_t* x, uint8_t* xs, size_t row_bytes) {
   __shared__ int ids[kMaxSmall];
   __shared__ int part[4][64];
   __shared__ int h[kMaxRouteExperts];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x;
-  const int at0 = blockIdx.y * 256 + tid;
-  V first{};
-  if (at0 < len) first = x[(size_t)t * len + at0];  // on its way while the rows are found
+  const size_t at0 = ((size_t)blockIdx.y * 256 + tid) * 16;
+  v4i first = {0, 0, 0, 0};  // on its way while the rows are found
+  if (at0 < row_bytes) load16(x + (size_t)t * row_bytes + at0, row_bytes - at0, first);
   for (int i = tid; i < a.n; i += 256) ids[i] = expert_of(a, i);
   const bool counts = t == 0 && blockIdx.y == 0;
   if (counts)
@@ -381,57 +403,55 @@ __global__ __launch_bounds__(256) void k_dispatch_small(DispatchArgs a, int topk
     if (blockIdx.y == 0) a.rows[t * topk + tid] = row;
   }
   __syncthreads();
-  for (int i = at0; i < len; i += gridDim.y * 256) {
-    const V v = i == at0 ? first : x[(size_t)t * len + i];
+  for (size_t i = at0; i < row_bytes; i += gridDim.y * 4096) {
+    v4i v = first;
+    if (i != at0) load16(x + (size_t)t * row_bytes + i, row_bytes - i, v);
     for (int s = 0; s < topk; s++) {
       const int r = part[0][s];
-      if (r >= 0) xs[(size_t)r * len + i] = v;
+      if (r >= 0) store16(xs + (size_t)r * row_bytes + i, row_bytes - i, v);
     }
   }
 }
 
 // ---- rows out and back ---------------------------------------------------------------
-template <typename V>
-__global__ __launch_bounds__(256) void k_gather(const V* x, const int32_t* rows, V* xs, int topk, int len) {
-  const int t = blockIdx.x, i = blockIdx.y * 256 + threadIdx.x;
-  if (i >= len) return;
-  const V v = x[(size_t)t * len + i];
+__global__ __launch_bounds__(256) void k_gather(const uint8_t* x, const int32_t* rows, uint8_t* xs, int topk, size_t row_bytes) {
+  const int t = blockIdx.x;
+  const size_t i = ((size_t)blockIdx.y * 256 + threadIdx.x) * 16;
+  if (i >= row_bytes) return;
+  v4i v;
+  load16(x + (size_t)t * row_bytes + i, row_bytes - i, v);
   for (int s = 0; s < topk; s++) {
     const int r = rows[(size_t)t * topk + s];
-    if (r >= 0) xs[(size_t)r * len + i] = v;
+    if (r >= 0) store16(xs + (size_t)r * row_bytes + i, row_bytes - i, v);
   }
 }
 
-template <int YT, int OT, int N>
+// 8 values a thread, at any address: rows of an odd length start anywhere (6276
+// tokens of 5 x 1055 bf16: 50.7 us one by one -> 30.2).
+template <int YT, int OT>
 __global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
-  const int t = blockIdx.x, i = (blockIdx.y * 256 + threadIdx.x) * N;
-  if (i >= a.hidden) return;
-  float sum[N];
-  if (a.add) load_n_as_f32<OT, N>(a.add, (size_t)t * a.hidden + i, sum);
-  else {
+  const int t = blockIdx.x, i = (blockIdx.y * 256 + threadIdx.x) * 8, left = a.hidden - i;
+  if (left <= 0) return;
+  float sum[8];
 #pragma unroll
-    for (int u = 0; u < N; u++) sum[u] = 0.0f;
-  }
+  for (int u = 0; u < 8; u++) sum[u] = 0.0f;
+  if (a.add) load_some_as_f32<OT>(a.add, (size_t)t * a.hidden + i, left, sum);
   for (int s = 0; s < a.topk; s++) {
     const size_t at = (size_t)t * a.topk + s;
     const int r = a.rows ? a.rows[at] : (unsigned)a.ids[at] < (unsigned)a.experts ? (int)at : -1;
     if (r < 0) continue;
-    const float w = a.weights[(size_t)t * a.topk + s];
-    float y[N];
-    load_n_as_f32<YT, N>(a.y, (size_t)r * a.hidden + i, y);
+    const float w = a.weights[at];
+    float y[8];
+    load_some_as_f32<YT>(a.y, (size_t)r * a.hidden + i, left, y);
 #pragma unroll
-    for (int u = 0; u < N; u++) sum[u] += w * y[u];
+    for (int u = 0; u < 8; u++) sum[u] += w * y[u];
   }
-  store_n_from_f32<OT, N>(a.out, (size_t)t * a.hidden + i, sum);
+  store_some_from_f32<OT>(a.out, (size_t)t * a.hidden + i, left, sum);
 }
 
 template <int YT, int OT>
 hipError_t combine_dt(const CombineArgs& a, hipStream_t st) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.add) | reinterpret_cast<uintptr_t>(a.out);
-  if (a.hidden % 8 == 0 && p % 16 == 0)
-    hipLaunchKernelGGL((k_combine<YT, OT, 8>), dim3(a.tokens, (a.hidden + 2047) / 2048), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_combine<YT, OT, 1>), dim3(a.tokens, (a.hidden + 255) / 256), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_combine<YT, OT>), dim3(a.tokens, (a.hidden + 2047) / 2048), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -493,20 +513,13 @@ hipError_t launch_dispatch_rows(const DispatchArgs& a, int topk, const void* x, 
   const bool small = a.n <= kMaxSmall && (long)a.n * topk <= 8 * kMaxSmall;
   if (!small)
     if (hipError_t e = launch_dispatch(a, st)) return e;
-  const uintptr_t p = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xs);
-  auto go = [&](auto v) {
-    using V = decltype(v);
-    const int len = (int)(row_bytes / sizeof(V));
-    const V* from = static_cast<const V*>(x);
-    V* to = static_cast<V*>(xs);
-    // few tokens: their rows are split over workgroups
-    const int parts = tokens >= 256 ? 1 : (len + 255) / 256;
-    if (small) hipLaunchKernelGGL((k_dispatch_small<V>), dim3(tokens, parts), dim3(256), 0, st, a, topk, from, to, len);
-    else hipLaunchKernelGGL((k_gather<V>), dim3(tokens, (len + 255) / 256), dim3(256), 0, st, from, a.rows, to, topk, len);
-  };
-  if (row_bytes % 16 == 0 && p % 16 == 0) go(v4i{});
-  else if (row_bytes % 4 == 0 && p % 4 == 0) go(uint32_t{});
-  else go(uint16_t{});
+  const uint8_t* from = static_cast<const uint8_t*>(x);
+  uint8_t* to = static_cast<uint8_t*>(xs);
+  const unsigned parts = (unsigned)((row_bytes + 4095) / 4096);
+  // (in one launch few tokens' rows are split over workgroups, many's are not: each
+  // counts the slots for itself)
+  if (small) hipLaunchKernelGGL(k_dispatch_small, dim3(tokens, tokens >= 256 ? 1 : parts), dim3(256), 0, st, a, topk, from, to, row_bytes);
+  else hipLaunchKernelGGL(k_gather, dim3(tokens, parts), dim3(256), 0, st, from, a.rows, to, topk, row_bytes);
   return hipGetLastError();
 }
 
