@@ -66,10 +66,10 @@ hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_
 // Streamed tiles keep the weights' way from HBM busy and cost a fetch of the
 // weights for each; the others cost rounds of the CUs by a stage's time, in us,
 // as measured (a stage: one 128-block of K):
-//   64 rows    0.57 a stage up to 256 tiles, 0.9 for two on a CU; in f16 (f32
-//              results, SwiGLU) 0.85 and 1.2
-//   128 rows   1.6, f32 results only
-//   256 rows   1.05
+//   64 rows    0.41 a stage up to 256 tiles, 0.65 for two on a CU; in f16 0.8 and
+//              1.25 (SwiGLU 0.85 and 1.2)
+//   128 rows   1.8, f32 results only
+//   256 rows   1.05, from half of the CUs on more: the card's power, 1.5 for all
 // 1000 rows of 4096 -> 4096: 30 us with 64 rows and 38 with 256; 4096 rows 110 and
 // 80.  16 experts with 32 rows each run on 64-row tiles, which sum SwiGLU's products
 // in f16, from 48 rows on on 256-row tiles, which read each expert's weights once.
@@ -83,17 +83,18 @@ int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swigl
   if (each <= 16) return 16;
   // two fetches of small weights come from the cache
   if (each <= 32) return ((swiglu ? n * 2L : n) + 31) / 32 <= 192 ? 16 : 32;
-  const bool f16_sums = swiglu || c_dtype == MX_DTYPE_F32;
+  const bool f32 = !swiglu && c_dtype == MX_DTYPE_F32;
   const double kb = (k + kQBlock - 1) / kQBlock;
   auto rounds = [](long tiles, long at_once) { return (double)((tiles + at_once - 1) / at_once); };
   auto tiles = [&](long r, long c) { return groups * ((each + r - 1) / r) * ((n + c - 1) / c); };
   const long t64 = tiles(64, 128);
-  const double us64 = t64 <= 256 ? kb * (f16_sums ? 0.85 : 0.57) + 5
-                                 : rounds(t64, swiglu ? 256 : 512) * (kb * (f16_sums ? 1.2 : 0.9) + 5);
-  if (!swiglu && c_dtype == MX_DTYPE_F32) return rounds(tiles(128, 256), 256) * (kb * 1.6 + 6) < us64 ? 128 : 64;
-  // (after others, a last round for at most half of the CUs takes about half of one)
+  const double us64 = t64 <= 256 ? kb * (swiglu ? 0.85 : f32 ? 0.8 : 0.41) + 6
+                                 : rounds(t64, swiglu ? 256 : 512) * (kb * (swiglu ? 1.2 : f32 ? 1.25 : 0.65) + 5.5);
+  if (f32) return rounds(tiles(128, 256), 256) * (kb * 1.8 + 9) < us64 ? 128 : 64;
   const long t256 = tiles(256, swiglu ? 128 : 256), last = t256 % 256;
-  return (t256 / 256 + (last == 0 ? 0 : last <= 128 && t256 > 256 ? 0.55 : 1)) * (kb * 1.05 + 6) < us64 ? 256 : 64;
+  const double stage = t256 > 214 ? 1.5 : t256 > 150 ? 0.007 * (double)t256 : 1.05;
+  // (after others, a last round for at most half of the CUs takes about half of one)
+  return (t256 / 256 + (last == 0 ? 0 : last <= 128 && t256 > 256 ? 0.55 : 1)) * (kb * stage + 8) < us64 ? 256 : 64;
 }
 
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {

@@ -26,7 +26,10 @@
 // normally distributed values, far below a 16-bit result's rounding and the
 // format's own 2^-4.  f32 results, and the sums before SwiGLU on 64-row tiles, whose
 // time is the weights' way from HBM, widen the codes to f16 instead (WIDE), whose
-// products add in f32: about 1e-7 of the sum, for half the rate.
+// products add in f32: about 1e-7 of the sum, for half the rate.  A product that
+// adds to the one before it starts 54 cycles after it, where one that does not
+// starts after 16: four sums are kept going at once (1024 rows of 8192 -> 2048 to
+// f32: 60 -> 56 us).
 #include <type_traits>
 
 #include "mx_block.h"
@@ -57,9 +60,10 @@ __device__ __forceinline__ int place_key(int r) { return (r >> 1 & 1) | (r >> 3 
 
 // TN weight rows (SwiGLU: TN / 2 of gate and the same of up) x TM activation
 // rows, by WN x WM waves, over K (or one of g.splits parts) in stages of one
-// 128-block, NS of them in LDS.
+// 128-block, NS of them in LDS.  (With room for two of the waves on a SIMD the
+// compiler leaves the sums out of AGPRs, which the scaling cannot read.)
 template <int DT, bool DUAL, int TN, int TM, int WN, int WM, int NS, bool WIDE>
-__global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
+__global__ __launch_bounds__(64 * WN * WM, 2) void k_block_tile(BlockGemmArgs g) {
   constexpr int NW = WN * WM, CN = TN / WN, CM = TM / WM, NI = CN / 16, MJ = CM / 16;
   constexpr int SLOT = (TN + TM) * kQBlock, NDMA = (TN + TM) / 8 / NW, PER = NDMA + 1;
   constexpr int ND = DUAL ? 2 : 1;  // weight scales of a wave
@@ -224,7 +228,8 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   // same where they fit the registers, and spill here.)
   v8i wf[NI], af[2];
   v8h wh[WIDE ? NI : 1][4];
-  v4f t[NI];
+  constexpr int CH = WIDE && NI < 4 && NW == 4 ? 2 : 1;  // sums of a product's K quarters
+  v4f t[NI], t1[CH > 1 ? NI : 1];
   float sc[2][ND], av[2], ws[ND];
   auto column = [&](auto u, int j) __attribute__((always_inline)) {
     af[j & 1] = frag(slot(u) + TN * 128, arow(j));
@@ -237,10 +242,13 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
   };
   auto add = [&](int i, int j) __attribute__((always_inline)) {  // column j's sums
 #pragma unroll
-    for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(t[i][v], sc[j & 1][DUAL && i >= NI / 2 ? 1 : 0], acc[i][j][v]);
+    for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(CH > 1 ? t[i][v] + t1[i][v] : t[i][v], sc[j & 1][DUAL && i >= NI / 2 ? 1 : 0], acc[i][j][v]);
   };
 #pragma unroll
-  for (int i = 0; i < NI; i++) t[i] = v4f{0, 0, 0, 0};
+  for (int i = 0; i < NI; i++) {
+    t[i] = v4f{0, 0, 0, 0};
+    if (CH > 1) t1[i] = v4f{0, 0, 0, 0};
+  }
 #pragma unroll
   for (int d = 0; d < ND; d++) sc[1][d] = 0.0f;
   column(I0{}, 0);
@@ -275,22 +283,30 @@ __global__ __launch_bounds__(64 * WN * WM) void k_block_tile(BlockGemmArgs g) {
       }
       v8h xh[4];
       if constexpr (WIDE) widen4(af[j & 1], xh);
+      if constexpr (WIDE) {
+        // A quarter of K for all weight rows in turn, and with few of them two sums of
+        // each: a product waits for the end of the one that it adds to.
 #pragma unroll
-      for (int i = 0; i < NI; i++) {
-        add(i, (j + MC - 1) % MC);
-        if constexpr (WIDE) {
-          t[i] = v4f{0, 0, 0, 0};
+        for (int q = 0; q < 4; q++)
 #pragma unroll
-          for (int q = 0; q < 4; q++) t[i] = mfma_f16_16x16x32(wh[i][q], xh[q], t[i]);
-        } else {
+          for (int i = 0; i < NI; i++) {
+            if (q == 0) add(i, (j + MC - 1) % MC);
+            v4f& sum = q % CH ? t1[i] : t[i];
+            sum = mfma_f16_16x16x32(wh[i][q], xh[q], q < CH ? v4f{0, 0, 0, 0} : sum);
+            if (j == MC - 1 && q == 0) weights(Next{}, i);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          add(i, (j + MC - 1) % MC);
           t[i] = mfma_fp8_16x16x128(wf[i], af[j & 1]);
+          if (j == MC - 1) weights(Next{}, i);
         }
-        if (j == MC - 1) weights(Next{}, i);
       }
 #pragma unroll
-      for (int i = 0; i < NI; i++) {
+      for (int i = 0; i < (WIDE ? 4 : 1) * NI; i++) {
         __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
-        __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         if (j == MC - 1) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
         else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
