@@ -70,9 +70,10 @@ hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_
 //              1.25 (SwiGLU 0.85 and 1.2)
 //   128 rows   1.8, f32 results only
 //   256 rows   1.05, from half of the CUs on more: the card's power, 1.5 for all
-// 1000 rows of 4096 -> 4096: 30 us with 64 rows and 38 with 256; 4096 rows 110 and
-// 80.  16 experts with 32 rows each run on 64-row tiles, which sum SwiGLU's products
-// in f16, from 48 rows on on 256-row tiles, which read each expert's weights once.
+// 1645 rows of 7680 -> 9728: 191 us with 64 rows and 172 with 256; to f32, 1381 rows
+// of 512 -> 6144 26 us with 64 rows and 31 with 128.  16 experts with 32 rows each
+// run on 64-row tiles, which sum SwiGLU's products in f16, from 48 rows on on 256-row
+// tiles, which read each expert's weights once.
 int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swiglu) {
   const long each = (rows + groups - 1) / groups;
   if (groups > 1) {  // experts differ in rows: room for more than the mean
