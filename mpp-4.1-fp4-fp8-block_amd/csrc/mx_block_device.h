@@ -61,17 +61,19 @@ __device__ __forceinline__ void widen4(const v8i& w, v8h* h) {
   for (int q = 0; q < 4; q++) h[q] = fp8x8_to_f16<BK_E4M3>((uint32_t)w[2 * q], (uint32_t)w[2 * q + 1]);
 }
 
-// `left` of four values; whole: all four, aligned to their size
+// `left` of four values, at any address of their type (rows of an odd length start
+// anywhere)
 template <int DT>
-__device__ __forceinline__ void store4(void* p, size_t i, v4f v, int left, bool whole) {
-  if (whole) {
-    if (left <= 0) return;
+__device__ __forceinline__ void store4(void* p, size_t i, v4f v, int left) {
+  if (left >= 4) {
     if constexpr (DT == MX_DTYPE_F32) {
-      *reinterpret_cast<v4f*>(static_cast<float*>(p) + i) = v;
+      __builtin_memcpy(static_cast<float*>(p) + i, &v, 16);
     } else if constexpr (DT == MX_DTYPE_F16) {
-      *reinterpret_cast<v4h*>(static_cast<_Float16*>(p) + i) = v4h{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+      const v4h h{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+      __builtin_memcpy(static_cast<_Float16*>(p) + i, &h, 8);
     } else {
-      *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p) + i) = v4bf{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      const v4bf h{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      __builtin_memcpy(static_cast<__bf16*>(p) + i, &h, 8);
     }
     return;
   }

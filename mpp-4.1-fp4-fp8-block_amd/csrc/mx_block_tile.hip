@@ -371,7 +371,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_block_tile(BlockGemmArgs g)
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int c = n0 + wrow(i) + kq * 4;
-        store4<DT>(g.c, ((size_t)sp * g.m + row0 + r) * g.n + c, acc[i][j], g.n - c, g.n % 4 == 0);
+        store4<DT>(g.c, ((size_t)sp * g.m + row0 + r) * g.n + c, acc[i][j], g.n - c);
       }
     }
   }
