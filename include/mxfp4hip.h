@@ -347,6 +347,7 @@ int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const 
  *            with its experts' block scales one after the other.
  *   add      [tokens][hidden] or NULL, added to the sum (a shared expert's rows).
  *   out      [tokens][hidden] in dtype; may be add.
+ * The experts' rows and their weighted sum are f32, rounded once to out.
  * 1 <= n_experts <= 512; hidden, intermediate % 16 and <= 65536; cfg->tokens = 0 is
  * allowed. */
 int mx_moe_block_forward(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, int topk, const void* x,

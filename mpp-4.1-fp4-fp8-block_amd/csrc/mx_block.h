@@ -81,6 +81,7 @@ struct BlockGemmArgs {
   void* c;                           // [m][n]; SwiGLU: E4M3 codes, and
   float* c_s;                        // their scales [n / 128][m]
   int m, n, k;
+  int fp8_cores;                     // f32 results by tiles: the FP8 cores' sums will do
   int tile_rows;                     // block_tile_rows
   int splits;                        // parts of K (block_splits): more than one are summed from
   void* part;                        // f32 [splits][m][n]
