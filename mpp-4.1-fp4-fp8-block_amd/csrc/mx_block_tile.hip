@@ -45,8 +45,11 @@ namespace {
 constexpr int kCUs = 256;           // of an MI355X, 32 in each of 8 XCDs
 constexpr int kPast = 0x7fffff00;  // past every resource's range
 constexpr int lgkm0_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4); }
-__device__ __forceinline__ void dma16(v4i rsrc, void* lds, int lane_offset, int offset) {
-  llvm_amdgcn_raw_buffer_load_lds_u32(rsrc, (lds_u32)lds, 16, lane_offset, offset, 0, 0);
+// The resource from `offset` bytes on, of those that it has.  (An instruction's scalar
+// offset would not be checked against the range.)
+__device__ __forceinline__ v4i rsrc_from(v4i rsrc, int offset) {
+  const uint64_t a = ((uint64_t)(uint32_t)rsrc[1] << 32 | (uint32_t)rsrc[0]) + (uint32_t)offset;
+  return v4i{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), rsrc[2] - offset, rsrc[3]};
 }
 __device__ __forceinline__ void dma4(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, lds, 4, 0, 0); }
 
@@ -127,18 +130,21 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_block_tile(BlockGemmArgs g)
   // DMA: an instruction moves 8 rows of 128 bytes, 16-byte chunk c of row r to
   // place c ^ place_key(r).
   // Through buffer resources of the tile's rows (of a whole batch whose rows are
-  // picked): what lies past them reads as zero.  So do chunks past K, on both
-  // sides: what lies there may be NaN.
+  // picked), with the row in the lane's offset: what lies past them reads as zero.
+  // So do chunks past K, on both sides: what lies there may be NaN.
   const int skip = kb0 * kQBlock, tail = min(kQBlock, K - skip - (KB - 1) * kQBlock) / 16;  // chunks of the last block
   const int chunk = (lane & 7) ^ place_key((wave & 1) * 8 + (lane >> 3));
   static_assert(NW % 2 == 0, "a wave's groups of 8 rows are all even or all odd");
   constexpr int TW = TN / ND, QW = TN / 8 / NW, QA = NDMA - QW;  // weight rows of a matrix; instructions of a wave
-  static_assert(TN / 8 % NW == 0, "whole instructions");
+  static_assert(QW % ND == 0 && TN / 8 % NW == 0, "whole instructions");
   // wave w moves weight rows (q NW + w) 8 ..: with SwiGLU, the first half of q gate
   const uint32_t wrange = (uint32_t)min(TW, g.n - n0) * (uint32_t)K - skip;
   const size_t wo = expert * g.w_stride + (size_t)n0 * K + skip;
   const v4i wrs0 = rsrc_of<true>(g.w0 + wo, wrange), wrs1 = rsrc_of<true>((DUAL ? g.w1 : g.w0) + wo, wrange);
-  const int woff = (wave * 8 + (lane >> 3)) * K + chunk * 16;
+  constexpr int QM = QW / ND;  // instructions of a matrix
+  int woff[QM];
+#pragma unroll
+  for (int q = 0; q < QM; q++) woff[q] = ((q * NW + wave) * 8 + (lane >> 3)) * K + chunk * 16;
   const v4i ars = rsrc_of<true>((g.src ? g.a : g.a + (size_t)row0 * K) + skip, (uint32_t)(g.src ? g.a_rows : rows) * (uint32_t)K - skip);
   int aoff[QA];
 #pragma unroll
@@ -166,15 +172,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_block_tile(BlockGemmArgs g)
     uint8_t* s = slot(u);
     // (no branch: the compiler would move products past it)
     const bool zero = (k >= KB) | ((k == KB - 1) & (chunk >= tail));
-    const int ko = k * kQBlock;
+    const int ko = min(k, KB - 1) * kQBlock;
 #pragma unroll
-    for (int q = p * QW / PARTS; q < (p + 1) * QW / PARTS; q++) {
-      const bool up = DUAL && q >= QW / 2;
-      dma16(up ? wrs1 : wrs0, s + (q * NW + wave) * 1024, zero ? kPast : woff, ko + (up ? q - QW / 2 : q) * NW * 8 * K);
-    }
+    for (int q = p * QW / PARTS; q < (p + 1) * QW / PARTS; q++)
+      buffer_dma16(rsrc_from(q >= QM ? wrs1 : wrs0, ko), s + (q * NW + wave) * 1024, zero ? kPast : woff[q % QM]);
 #pragma unroll
     for (int q = p * QA / PARTS; q < (p + 1) * QA / PARTS; q++)
-      dma16(ars, s + TN * 128 + (q * NW + wave) * 1024, zero ? kPast : aoff[q], ko);
+      buffer_dma16(rsrc_from(ars, ko), s + TN * 128 + (q * NW + wave) * 1024, zero ? kPast : aoff[q]);
     if (p == PARTS - 1) dma4(ssrc + (size_t)min(k, KB - 1) * g.a_rows, aslot(u) + (wave * 64) % TM);
   };
   auto issue_all = [&](int k, auto u) {
