@@ -74,7 +74,7 @@ int ensure_ws(mx_ctx* c, size_t bytes) {
   if (hipStreamIsCapturing(c->stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone)
     return set_err(c, MX_EINVAL,
                    "The workspace must grow to %zu bytes, which is not allowed while the stream is being "
-                   "captured: run one forward of the largest shape before capturing.", bytes);
+                   "captured: run this call once before capturing.", bytes);
   if (c->ws) {
     MX_HIP(c, hipStreamSynchronize(c->stream));
     MX_HIP(c, hipFree(c->ws));
@@ -1072,7 +1072,8 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
   const size_t bh = (H + mx::kQBlock - 1) / mx::kQBlock, bi = (I + mx::kQBlock - 1) / mx::kQBlock;
   const int gu_rows = mx::block_tile_rows(T, 1, I, H, MX_DTYPE_F16, true);
   const bool few = mx::block_streams(gu_rows);  // the middle comes in f32; else in its codes
-  const size_t o_xq = take((size_t)T * H), o_xs = take(T * bh * 4), o_mid = take(few ? (size_t)T * I * 4 : 0),
+  // (room for the most streamed tokens whenever there are more: the need falls with none)
+  const size_t o_xq = take((size_t)T * H), o_xs = take(T * bh * 4), o_mid = take((size_t)std::min<long>(T, mx::block_stream_most(1)) * I * 4),
                o_mq = take((size_t)T * I), o_ms = take(T * bi * 4);
   if (int rc = ensure_ws(c, off)) return rc;
   uint8_t* ws = static_cast<uint8_t*>(c->ws);

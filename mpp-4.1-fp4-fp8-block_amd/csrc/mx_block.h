@@ -65,6 +65,18 @@ struct CombineArgs {
 };
 hipError_t launch_combine(int y_dtype, int out_dtype, const CombineArgs& a, hipStream_t st);
 
+// Workspace of mx_moe_block_forward: offsets of its parts, 256-byte aligned.  Every
+// part takes no less for more tokens (or more of anything), whichever kernels run.
+struct ExpertsLayout {
+  size_t xq, xs;                     // [T][H] codes of x, [H / 128][T] scales
+  size_t rows, src, counts, tiles, n_tiles, hist;
+  size_t mid;                        // f32 middles, of as many slots as streams take
+  size_t mq, ms;                     // [n][I] codes of the middle, [I / 128][n] scales
+  size_t y;                          // f32 [n][H] experts' rows
+  size_t total;
+};
+ExpertsLayout experts_layout(int T, int H, int I, int E, int topk);
+
 // ---- block-scaled FP8 (mx_block.hip) ------------------------------------------
 hipError_t launch_block_quantize(int dtype, const void* src, int rows, int k, uint8_t* q, float* scales,
                                  hipStream_t st);
@@ -102,9 +114,15 @@ struct BlockGemmArgs {
 // (weights streamed), 64, 128 (f32 results) or 256.
 int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swiglu);
 int block_splits(int m, int n, int k, int tile_rows);
+// Bytes of the parts of any product of up to m rows: no less for more of m, n or k,
+// so that a workspace of the largest product holds the others' (a call that grew it
+// would free what a captured call still points at).
+size_t block_split_bytes(int m, int n, int k);
 // The product by tiles of g.tile_rows rows.  SwiGLU: streamed tiles write
 // f32 [m][n] to c, larger ones E4M3 codes to c and their scales to c_s.
 inline bool block_streams(int tile_rows) { return tile_rows <= 32; }
+// The most rows in `groups` matrices that block_tile_rows gives to streams.
+inline long block_stream_most(int groups) { return groups > 1 ? 20L * groups : 32; }
 hipError_t launch_block_gemm(int c_dtype, const BlockGemmArgs& g, hipStream_t st);
 hipError_t launch_block_stream(int c_dtype, const BlockGemmArgs& g, hipStream_t st);  // mx_block_stream.hip
 // One token, k <= kMaxDirect: gate/up products of an f16 or bf16 row or the down

@@ -78,7 +78,7 @@ int block_tile_rows(long rows, int groups, int n, int k, int c_dtype, bool swigl
   const long each = (rows + groups - 1) / groups;
   if (groups > 1) {  // experts differ in rows: room for more than the mean
     if (each <= 6) return 16;
-    if (each <= 20) return 32;
+    if (each <= 20) return 32;  // (block_stream_most)
     if (swiglu) return each <= 48 ? 64 : 256;
   }
   if (each <= 16) return 16;

@@ -449,6 +449,13 @@ int block_splits(int m, int n, int k, int tile_rows) {
   return (int)(s < most ? s : most > 1 ? most : 1);
 }
 
+// At most 256 tiles' f32 sums, and one part for every four blocks of K.
+size_t block_split_bytes(int m, int n, int k) {
+  const long parts = (k + kQBlock - 1) / kQBlock / 4;
+  const double all = 4.0 * parts * m * n, tiles = 4.0 * 256 * 64 * 128;
+  return m <= 32 || parts <= 1 ? 0 : (size_t)(all < tiles ? all : tiles);
+}
+
 hipError_t launch_block_tile(int c_dtype, const BlockGemmArgs& g, hipStream_t st) {
   if (g.w1)
     return g.tile_rows == 256 ? launch_one<MX_DTYPE_F32, true, 256, 256, 4, 2, 2, false>(g, st)

@@ -13,6 +13,31 @@ hipStream_t mx_ctx_stream(mx_ctx* c);
 int mx_ctx_error(mx_ctx* c, int code, const char* message);
 int mx_ctx_workspace(mx_ctx* c, size_t bytes, void** p);
 
+namespace mx {
+
+ExpertsLayout experts_layout(int T, int H, int I, int E, int topk) {
+  const size_t n = (size_t)T * topk, used = n < (size_t)E ? n : E, few = (size_t)block_stream_most(E);
+  auto blocks = [](int k) { return (size_t)((k + kQBlock - 1) / kQBlock); };
+  ExpertsLayout l{};
+  auto take = [&](size_t bytes) { const size_t o = l.total; l.total = (o + bytes + 255) / 256 * 256; return o; };
+  l.xq = take((size_t)T * H);
+  l.xs = take(T * blocks(H) * 4);
+  l.rows = take(n * 4);
+  l.src = take(n * 4);
+  l.counts = take((size_t)E * 4);
+  l.tiles = take((used + n / 16) * sizeof(RowTile));  // tiles have 16 rows at least
+  l.n_tiles = take(4);
+  l.hist = take(dispatch_ws_bytes((int)n, E));
+  const size_t mids = n < few ? n : few;
+  l.mid = take((mids > (size_t)topk ? mids : topk) * I * 4);  // (one token's slots are not split)
+  l.mq = take(n * I);
+  l.ms = take(n * blocks(I) * 4);
+  l.y = take(n * H * 4);
+  return l;
+}
+
+}  // namespace mx
+
 namespace {
 
 int fail(mx_ctx* c, int code, const char* fmt, ...) {
@@ -52,9 +77,9 @@ int check_experts(mx_ctx* c, int experts) {
 // quantized where they are used.
 int block_experts_of_one(mx_ctx* c, int H, int I, int E, int topk, const void* x, int dtype, const int32_t* ids,
                          const float* weights, const mx_mlp_weights* w, const void* add, void* out) {
-  const size_t mid = ((size_t)topk * I * 4 + 255) / 256 * 256;
+  const mx::ExpertsLayout l = mx::experts_layout(1, H, I, E, topk);
   void* p = nullptr;
-  if (int rc = mx_ctx_workspace(c, mid + (size_t)topk * H * 4, &p)) return rc;
+  if (int rc = mx_ctx_workspace(c, l.total, &p)) return rc;
   uint8_t* ws = static_cast<uint8_t*>(p);
   hipStream_t st = mx_ctx_stream(c);
   mx::BlockGemmArgs g{};
@@ -69,20 +94,20 @@ int block_experts_of_one(mx_ctx* c, int H, int I, int E, int topk, const void* x
   g.s1 = static_cast<const float*>(w->up.scales);
   g.w_stride = (size_t)I * H;
   g.s_stride = (size_t)blocks(I) * blocks(H);
-  g.c = ws;
+  g.c = ws + l.mid;
   g.n = I;
   g.k = H;
   MX_RUN(c, mx::launch_block_direct(dtype, g, st));
-  g.raw = ws;
+  g.raw = ws + l.mid;
   g.row_per_slot = 1;
   g.w0 = static_cast<const uint8_t*>(w->down.data);
   g.w1 = nullptr;
   g.s0 = static_cast<const float*>(w->down.scales);
-  g.c = ws + mid;
+  g.c = ws + l.y;
   g.n = H;
   g.k = I;
   MX_RUN(c, mx::launch_block_direct(MX_DTYPE_F32, g, st));
-  const mx::CombineArgs b{ws + mid, nullptr, weights, add, out, 1, topk, H, ids, E};
+  const mx::CombineArgs b{ws + l.y, nullptr, weights, add, out, 1, topk, H, ids, E};
   MX_RUN(c, mx::launch_combine(MX_DTYPE_F32, dtype, b, st));
   return MX_OK;
 }
@@ -91,8 +116,6 @@ int block_experts_of_one(mx_ctx* c, int H, int I, int E, int topk, const void* x
 int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x, int dtype, const int32_t* ids,
                   const float* weights, const mx_mlp_weights* w, const void* add, void* out) {
   const int n = T * topk;
-  size_t off = 0;
-  auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
   // one tile height for both products, so that they share the list of tiles
   const int used = n < E ? n : E, tile_rows = mx::block_tile_rows(n, used, I, H, dtype, true), max_tiles = used + n / tile_rows;
   // Few rows write the middle in f32 first, more of them its codes alone.  The
@@ -101,28 +124,25 @@ int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x
   // would leave their roundings.  (Rows of 16 bits take half the bytes: 4096 tokens,
   // top 8 of 64 x (7168, 2048), 1870 us instead of 2010; 256 tokens 567 and 575.)
   const bool few = mx::block_streams(tile_rows);
-  const size_t o_xq = take((size_t)T * H), o_xs = take((size_t)T * blocks(H) * 4), o_rows = take((size_t)n * 4),
-               o_src = take((size_t)n * 4), o_counts = take((size_t)E * 4), o_tiles = take((size_t)max_tiles * sizeof(mx::RowTile)),
-               o_nt = take(4), o_hist = take(mx::dispatch_ws_bytes(n, E)), o_mid = take(few ? (size_t)n * I * 4 : 0),
-               o_mq = take((size_t)n * I), o_ms = take((size_t)n * blocks(I) * 4), o_y = take((size_t)n * H * 4);
+  const mx::ExpertsLayout l = mx::experts_layout(T, H, I, E, topk);
   void* p = nullptr;
-  if (int rc = mx_ctx_workspace(c, off, &p)) return rc;
+  if (int rc = mx_ctx_workspace(c, l.total, &p)) return rc;
   uint8_t* ws = static_cast<uint8_t*>(p);
   hipStream_t st = mx_ctx_stream(c);
-  mx::DispatchArgs d{ids, n, E, reinterpret_cast<int32_t*>(ws + o_counts), reinterpret_cast<int32_t*>(ws + o_rows),
-                     reinterpret_cast<int32_t*>(ws + o_src), reinterpret_cast<mx::RowTile*>(ws + o_tiles),
-                     reinterpret_cast<int32_t*>(ws + o_nt), tile_rows, reinterpret_cast<int32_t*>(ws + o_hist)};
-  MX_RUN(c, mx::launch_prepare(d, dtype, x, T, H, ws + o_xq, reinterpret_cast<float*>(ws + o_xs), st));
+  mx::DispatchArgs d{ids, n, E, reinterpret_cast<int32_t*>(ws + l.counts), reinterpret_cast<int32_t*>(ws + l.rows),
+                     reinterpret_cast<int32_t*>(ws + l.src), reinterpret_cast<mx::RowTile*>(ws + l.tiles),
+                     reinterpret_cast<int32_t*>(ws + l.n_tiles), tile_rows, reinterpret_cast<int32_t*>(ws + l.hist)};
+  MX_RUN(c, mx::launch_prepare(d, dtype, x, T, H, ws + l.xq, reinterpret_cast<float*>(ws + l.xs), st));
   mx::BlockGemmArgs g{};
-  g.a = ws + o_xq;
-  g.a_s = reinterpret_cast<float*>(ws + o_xs);
+  g.a = ws + l.xq;
+  g.a_s = reinterpret_cast<float*>(ws + l.xs);
   g.a_rows = T;
   g.w0 = static_cast<const uint8_t*>(w->gate.data);
   g.w1 = static_cast<const uint8_t*>(w->up.data);
   g.s0 = static_cast<const float*>(w->gate.scales);
   g.s1 = static_cast<const float*>(w->up.scales);
-  g.c = few ? ws + o_mid : ws + o_mq;
-  g.c_s = reinterpret_cast<float*>(ws + o_ms);
+  g.c = few ? ws + l.mid : ws + l.mq;
+  g.c_s = reinterpret_cast<float*>(ws + l.ms);
   g.m = n;
   g.n = I;
   g.k = H;
@@ -137,20 +157,20 @@ int block_experts(mx_ctx* c, int T, int H, int I, int E, int topk, const void* x
   g.src_div = topk;
   MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
   if (few)
-    MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + o_mid, n, I, ws + o_mq, reinterpret_cast<float*>(ws + o_ms), st));
-  g.a = ws + o_mq;
-  g.a_s = reinterpret_cast<float*>(ws + o_ms);
+    MX_RUN(c, mx::launch_block_quantize(MX_DTYPE_F32, ws + l.mid, n, I, ws + l.mq, reinterpret_cast<float*>(ws + l.ms), st));
+  g.a = ws + l.mq;
+  g.a_s = reinterpret_cast<float*>(ws + l.ms);
   g.a_rows = n;
   g.w0 = static_cast<const uint8_t*>(w->down.data);
   g.w1 = nullptr;
   g.s0 = static_cast<const float*>(w->down.scales);
-  g.c = ws + o_y;
+  g.c = ws + l.y;
   g.n = H;
   g.k = I;
   g.src = nullptr;
   g.fp8_cores = 1;
   MX_RUN(c, mx::launch_block_gemm(MX_DTYPE_F32, g, st));
-  const mx::CombineArgs b{ws + o_y, d.rows, weights, add, out, T, topk, H, nullptr, 0};
+  const mx::CombineArgs b{ws + l.y, d.rows, weights, add, out, T, topk, H, nullptr, 0};
   MX_RUN(c, mx::launch_combine(MX_DTYPE_F32, dtype, b, st));
   return MX_OK;
 }
@@ -275,8 +295,8 @@ int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const ui
   g.k = k;
   g.tile_rows = mx::block_tile_rows(m, 1, n, k, c_dtype, false);
   g.splits = mx::block_splits(m, n, k, g.tile_rows);
-  if (g.splits > 1)
-    if (int rc = mx_ctx_workspace(c, (size_t)g.splits * m * n * 4, &g.part)) return rc;
+  if (const size_t bytes = mx::block_split_bytes(m, n, k))
+    if (int rc = mx_ctx_workspace(c, bytes, &g.part)) return rc;
   MX_RUN(c, mx::launch_block_gemm(c_dtype, g, mx_ctx_stream(c)));
   return MX_OK;
 }
