@@ -326,15 +326,17 @@ int mx_moe_combine(mx_ctx* ctx, int tokens, int topk, int hidden, const void* y,
 /* Activations to E4M3 with one f32 scale per row and 128 values: src [rows][k]
  * (f32, f16, bf16) -> q [rows][k], scales [ceil(k/128)][rows].  scale =
  * amax * (1/448 in f32), at least 2^-126, 1 where all 128 are zero; code =
- * E4M3(x / scale), an f32 division, to nearest even.  128 values with a NaN or an infinity among them come out
- * as NaN.  k % 16 == 0, k <= 65536; rows = 0 is allowed. */
+ * E4M3(x / scale), an f32 division, to nearest even.  128 values with a NaN or
+ * an infinity among them come out as NaN.  k % 16 == 0, k <= 65536, rows <
+ * 2^28; rows = 0 is allowed. */
 int mx_block_quantize(mx_ctx* ctx, const void* src, int src_dtype, int rows, int k, uint8_t* q, float* scales);
 /* C[m][n] = sum over 128-blocks kb of a_scales[kb][m] * b_scales[n/128][kb] *
  * sum_{k in kb} A[m][k] * B[n][k], with A as mx_block_quantize and B [n][k] as
  * mx_fmt_quantize(MX_WFMT_FP8_BLOCK) writes them; f32 sums, C f32, f16 or
  * bf16.  f16 and bf16 results of more than 32 rows come from the FP8 matrix cores,
  * whose sums hold about 1e-5 of their value; f32 results and few rows from f16
- * products with f32 sums.  Any n >= 1, k % 16 == 0, k <= 65536; m = 0 is allowed. */
+ * products with f32 sums.  n >= 1, m and n < 2^28, k % 16 == 0, k <= 65536; m = 0
+ * is allowed. */
 int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const uint8_t* b,
                     const float* b_scales, void* c, int c_dtype, int m, int n, int k);
 /* The MLP of each token's experts with block-scaled FP8 weights, from token

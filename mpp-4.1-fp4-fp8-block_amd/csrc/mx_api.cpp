@@ -1058,8 +1058,8 @@ static int build_block_steps(mx_ctx* c, const mx_mlp_config* cfg, const void* x,
   if (cfg->tokens == 0 || cfg->hidden == 0 || cfg->intermediate == 0 || cfg->hidden % 16 || cfg->intermediate % 16)
     return set_err(c, MX_EINVAL, "Block FP8 needs hidden and intermediate to be positive multiples of 16, and tokens.");
   constexpr uint32_t kMost = mx::kMaxBlocks * mx::kQBlock;
-  if (cfg->tokens > 0x7fffffffu || cfg->hidden > kMost || cfg->intermediate > kMost)
-    return set_err(c, MX_EINVAL, "Block FP8 hidden and intermediate are at most %u.", kMost);
+  if (cfg->tokens >= (uint32_t)mx::kMaxRows || cfg->hidden > kMost || cfg->intermediate > kMost)
+    return set_err(c, MX_EINVAL, "Block FP8 hidden and intermediate are at most %u, and tokens below %d.", kMost, mx::kMaxRows);
   if (!x || !w || !out || !aligned16(x) || !aligned16(out))
     return set_err(c, MX_EINVAL, "MLP buffers must be non-null and 16-byte aligned.");
   const mx_qmatrix* mats[3] = {&w->gate, &w->up, &w->down};

@@ -5,6 +5,10 @@
 namespace mx {
 namespace {
 
+// Tokens of one launch: a grid holds 2^32 threads in x, and a token takes up to 256.
+constexpr int kMostTokens = 1 << 23;
+size_t dtype_size(int dtype) { return dtype == MX_DTYPE_F32 ? 4 : 2; }
+
 // ---- lanes ----------------------------------------------------------------------
 // DPP: lane ^ 1, lane ^ 2, 7 - lane of 8, 15 - lane of 16.  After as many of them as
 // log2(L), every lane of L has what the L lanes have together.
@@ -451,8 +455,19 @@ __global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
 
 template <int YT, int OT>
 hipError_t combine_dt(const CombineArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((k_combine<YT, OT>), dim3(a.tokens, (a.hidden + 2047) / 2048), dim3(256), 0, st, a);
-  return hipGetLastError();
+  const unsigned parts = ((unsigned)a.hidden + 2047) / 2048;
+  for (int t = 0; t < a.tokens; t += kMostTokens) {
+    CombineArgs p = a;
+    p.tokens = a.tokens - t < kMostTokens ? a.tokens - t : kMostTokens;
+    const size_t slot = (size_t)t * a.topk, out = (size_t)t * a.hidden * dtype_size(OT);
+    if (a.rows) p.rows += slot;  // (without, the slots of one token)
+    p.weights += slot;
+    p.out = static_cast<uint8_t*>(a.out) + out;
+    if (a.add) p.add = static_cast<const uint8_t*>(a.add) + out;
+    hipLaunchKernelGGL((k_combine<YT, OT>), dim3(p.tokens, parts), dim3(256), 0, st, p);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 template <int YT>
@@ -467,13 +482,25 @@ hipError_t combine_y(int out_dtype, const CombineArgs& a, hipStream_t st) {
 
 }  // namespace
 
-hipError_t launch_route(int dtype, const RouteArgs& a, hipStream_t st) {
+static hipError_t route_part(int dtype, const RouteArgs& a, hipStream_t st) {
   switch (dtype) {
     case MX_DTYPE_F32: return route_dt<MX_DTYPE_F32>(a, st);
     case MX_DTYPE_F16: return route_dt<MX_DTYPE_F16>(a, st);
     case MX_DTYPE_BF16: return route_dt<MX_DTYPE_BF16>(a, st);
   }
   return hipErrorInvalidValue;
+}
+
+hipError_t launch_route(int dtype, const RouteArgs& a, hipStream_t st) {
+  for (int t = 0; t < a.tokens; t += kMostTokens) {
+    RouteArgs p = a;
+    p.tokens = a.tokens - t < kMostTokens ? a.tokens - t : kMostTokens;
+    p.logits = static_cast<const uint8_t*>(a.logits) + (size_t)t * a.stride * dtype_size(dtype);
+    p.ids += (size_t)t * a.topk;
+    p.weights += (size_t)t * a.topk;
+    if (hipError_t e = route_part(dtype, p, st)) return e;
+  }
+  return hipSuccess;
 }
 
 static int chunks_of(int n) { return n > 0 ? (n + kChunk - 1) / kChunk : 1; }
@@ -518,9 +545,16 @@ hipError_t launch_dispatch_rows(const DispatchArgs& a, int topk, const void* x, 
   const unsigned parts = (unsigned)((row_bytes + 4095) / 4096);
   // (in one launch few tokens' rows are split over workgroups, many's are not: each
   // counts the slots for itself)
-  if (small) hipLaunchKernelGGL(k_dispatch_small, dim3(tokens, tokens >= 256 ? 1 : parts), dim3(256), 0, st, a, topk, from, to, row_bytes);
-  else hipLaunchKernelGGL(k_gather, dim3(tokens, parts), dim3(256), 0, st, from, a.rows, to, topk, row_bytes);
-  return hipGetLastError();
+  if (small) {
+    hipLaunchKernelGGL(k_dispatch_small, dim3(tokens, tokens >= 256 ? 1 : parts), dim3(256), 0, st, a, topk, from, to, row_bytes);
+    return hipGetLastError();
+  }
+  for (int t = 0; t < tokens; t += kMostTokens) {
+    hipLaunchKernelGGL(k_gather, dim3(tokens - t < kMostTokens ? tokens - t : kMostTokens, parts), dim3(256), 0, st,
+                       from + (size_t)t * row_bytes, a.rows + (size_t)t * topk, to, topk, row_bytes);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_combine(int y_dtype, int out_dtype, const CombineArgs& a, hipStream_t st) {

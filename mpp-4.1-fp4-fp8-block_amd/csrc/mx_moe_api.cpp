@@ -264,6 +264,7 @@ int mx_block_quantize(mx_ctx* c, const void* src, int src_dtype, int rows, int k
   if (!c) return MX_EINVAL;
   if (rows < 0 || k <= 0 || k % 16) return fail(c, MX_EINVAL, "block quantize needs rows >= 0 and k a positive multiple of 16.");
   if (k > mx::kMaxBlocks * mx::kQBlock) return fail(c, MX_EINVAL, "block quantize k is at most %d.", mx::kMaxBlocks * mx::kQBlock);
+  if (rows >= mx::kMaxRows) return fail(c, MX_EINVAL, "block quantize rows must be below %d.", mx::kMaxRows);
   if (!is_float(src_dtype)) return fail(c, MX_EINVAL, "block quantize source must be f32, f16 or bf16.");
   if (rows == 0) return MX_OK;
   if (!src || !q || !scales || !is_aligned(src, 16) || !is_aligned(q, 16) || !is_aligned(scales, 4))
@@ -278,6 +279,7 @@ int mx_block_matmul(mx_ctx* c, const uint8_t* a, const float* a_scales, const ui
   if (m < 0 || n <= 0 || k <= 0 || k % 16)
     return fail(c, MX_EINVAL, "block matmul needs m >= 0, n > 0 and k a positive multiple of 16.");
   if (k > mx::kMaxBlocks * mx::kQBlock) return fail(c, MX_EINVAL, "block matmul k is at most %d.", mx::kMaxBlocks * mx::kQBlock);
+  if (m >= mx::kMaxRows || n >= mx::kMaxRows) return fail(c, MX_EINVAL, "block matmul m and n must be below %d.", mx::kMaxRows);
   if (!is_float(c_dtype)) return fail(c, MX_EINVAL, "block matmul C must be f32, f16 or bf16.");
   if (m == 0) return MX_OK;
   if (!a || !a_scales || !b || !b_scales || !out || !is_aligned(a, 16) || !is_aligned(b, 16) || !is_aligned(out, 16) ||
