@@ -25,6 +25,11 @@ def blocks(n):
     return -(-n // 128)
 
 
+def part(buf, i, nbytes):
+    """The i-th run of nbytes of a buffer."""
+    return M.DevBuf(buf.dev, buf.ptr + i * nbytes, nbytes)
+
+
 class Layer:
     """Random weights in f32, quantized on the device to both formats."""
 
@@ -39,8 +44,8 @@ class Layer:
             w = dev.upload(rng.normal(0, 1 / np.sqrt(k), (experts * n, k)).astype(np.float32))
             q, s = dev.alloc(experts * n * k), dev.alloc(experts * blocks(n) * blocks(k) * 4)
             for e in range(experts):  # a block's scale covers rows of one expert only
-                M.load().mx_fmt_quantize(dev.ctx, M.WFMT_FP8_BLOCK, w.offset(e * n * k * 4), n, k, q.offset(e * n * k),
-                                         s.offset(e * blocks(n) * blocks(k) * 4))
+                dev.fmt_quantize(M.WFMT_FP8_BLOCK, part(w, e, n * k * 4), n, k, part(q, e, n * k),
+                                 part(s, e, blocks(n) * blocks(k) * 4))
             fp8.append((q, s))
             p, e8 = dev.alloc(experts * n * k // 2), dev.alloc(experts * n * k // 32)
             dev.mxfp4_quantize(w, M.DT_F32, experts * n, k, p, e8)
