@@ -328,8 +328,9 @@ int mx_moe_block_forward(mx_ctx* c, const mx_mlp_config* cfg, int n_experts, int
     return fail(c, MX_EINVAL, "MoE rows must be 16-byte aligned, ids and weights 4-byte.");
   if (T == 1 && H <= mx::kMaxDirect && I <= mx::kMaxDirect)
     return block_experts_of_one(c, H, I, E, topk, x, dtype, ids, weights, w, add, out);
-  // The picked rows of x are addressed by 31 bits: larger batches in parts.
-  const int most = (int)(0x7fff0000u / (uint32_t)H);
+  // Larger batches in parts: a part's picked rows of x are addressed by 31 bits, and
+  // half of that keeps the f32 rows of its slots to 4 GB a slot of a token.
+  const int most = (int)(0x3fff0000u / (uint32_t)H);
   for (int t = 0; t < T; t += most) {
     const size_t row = (size_t)t * H * 2;
     const int rc = block_experts(c, T - t < most ? T - t : most, H, I, E, topk, static_cast<const uint8_t*>(x) + row, dtype,

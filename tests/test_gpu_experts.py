@@ -4,7 +4,7 @@ import pytest
 
 import block_ref as R
 import mxfp4hip as M
-from test_gpu_block import dequant, weights
+from test_gpu_block import dequant, expert_ref, weights
 
 pytestmark = pytest.mark.gpu
 H, B = M.DT_F16, M.DT_BF16
@@ -66,3 +66,25 @@ def test_rows_that_nearly_cancel(dev, dtype, t):
     size = np.abs(one) * (1 + 2 * R.HALF_ULP[dtype])
     tol = 2 * (R.HALF_ULP[dtype] * size * 1.01 + R.TINY[dtype]) + 8 * 2.0 ** 6 * R.EPS / 2 * size
     assert np.all(np.abs(diff - one) <= tol)
+
+
+def test_batches_in_parts(dev):
+    """16400 tokens of 65536: the last 17 are a part of their own."""
+    t, h, i, e, k = 16400, 65536, 32, 3, 2
+    rng = np.random.default_rng(0)
+    x, out = dev.alloc(t * h * 2), dev.alloc(t * h * 2)
+    dev.fill_normal(x, H, t * h, seed=1)
+    dev.memset(out, 0xff)
+    ids = rng.integers(-1, e, (t, k)).astype(np.int32)
+    w = rng.random((t, k)).astype(np.float32)
+    ws = [weights(dev, rng, e, n, kk, std=0.05) for n, kk in ((i, h), (i, h), (h, i))]
+    dev.moe_block_forward(t, h, i, e, k, x, H, dev.upload(ids), dev.upload(w), M.Device.weights(*[v[:2] for v in ws]), out)
+    some = np.r_[0, 1, 5000, 16381:16386, t - 1]
+
+    def rows(buf):
+        return np.concatenate([dev.download(buf.offset(int(r) * h * 2), np.float16, (1, h)) for r in some])
+
+    ref, err = expert_ref(rows(x), ids[some], w[some], ws, None, H, cores=True)
+    got = rows(out).astype(np.float64)
+    x.free(), out.free()
+    assert np.all(np.abs(got - ref) <= err)
