@@ -349,7 +349,10 @@ int mx_block_matmul(mx_ctx* ctx, const uint8_t* a, const float* a_scales, const 
  *            with its experts' block scales one after the other.
  *   add      [tokens][hidden] or NULL, added to the sum (a shared expert's rows).
  *   out      [tokens][hidden] in dtype; may be add.
- * The experts' rows and their weighted sum are f32, rounded once to out.
+ * The experts' rows and their weighted sum are f32, rounded once to out.  The
+ * sums of the down products of more than 20 rows an expert on average, and of the
+ * gate and up products of more than 48 (one expert: of larger batches), come from
+ * the FP8 matrix cores (see mx_block_matmul); the others from f16 products.
  * 1 <= n_experts <= 512; hidden, intermediate % 16 and <= 65536; cfg->tokens = 0 is
  * allowed. */
 int mx_moe_block_forward(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, int topk, const void* x,
@@ -381,7 +384,9 @@ int mx_fmt_quantize(mx_ctx* ctx, int wfmt, const float* w, int rows, int k, void
 /* MLP with format weights: mpp_mlp_h_fp8e4m3_f_n128 / _h_fp8e5m2_f_n128 /
  * h_i8_f / h_i4_f / i8_i8_i32 rows (MPPMLPKernels.metal:50-125) with scales.
  * hidden and intermediate % 32; the _F8X2 rows % 64; W8A8 % 128;
- * FP8_BLOCK % 16. */
+ * FP8_BLOCK % 16 and <= 65536, whose products of more than 32 tokens come from
+ * the FP8 matrix cores (see mx_block_matmul), gate and up only of larger batches.
+ * x and out are f16. */
 int mx_fmt_mlp_forward(mx_ctx* ctx, int wfmt, const mx_mlp_config* cfg, const void* x,
                        const mx_mlp_weights* w, void* out);
 /* Timed loop of the format rows, as mx_mlp_benchmark (kernel_us_out and

@@ -69,7 +69,7 @@ hipError_t launch_block_quantize_weights(const float* w, int rows, int k, uint8_
 //   64 rows    0.41 a stage up to 256 tiles, 0.65 for two on a CU; in f16 0.8 and
 //              1.25 (SwiGLU 0.85 and 1.2)
 //   128 rows   1.8, f32 results only
-//   256 rows   1.05, from half of the CUs on more: the card's power, 1.5 for all
+//   256 rows   1.05, from half of the CUs on more (L2, and a lower clock), 1.5 for all
 // 1645 rows of 7680 -> 9728: 191 us with 64 rows and 172 with 256; to f32, 1381 rows
 // of 512 -> 6144 26 us with 64 rows and 31 with 128.  16 experts with 32 rows each
 // run on 64-row tiles, which sum SwiGLU's products in f16, from 48 rows on on 256-row
