@@ -281,7 +281,7 @@ int mx_moe_benchmark(mx_ctx* ctx, const mx_mlp_config* cfg, int n_experts, const
 /* No counterpart in the reference.  From gate logits to mx_moe_forward's rows
  * and counts, and from its rows back to tokens.  All of it stays on the device
  * in stream order; tokens = 0 is allowed and does nothing else than to clear
- * the counts.  topk <= 64 and tokens * topk < 2^26. */
+ * the counts.  topk <= 64, tokens * topk < 2^26 and hidden < 2^28. */
 enum { MX_ROUTE_SOFTMAX = 0, MX_ROUTE_SIGMOID = 1 };
 typedef struct {
   uint32_t tokens, experts, topk;   /* experts <= 512, topk <= 64 */
@@ -378,7 +378,8 @@ int mx_load_mxfp4(mx_ctx* ctx, const char* path, const char* blocks_name, const 
 
 /* ---- weight-format rows (config 3) ------------------------------------------ */
 /* Quantize f32 weights [rows][k] into format `wfmt` (scales per the enum;
- * the _F8X2 codes quantize as their FP8 format).  k % 32; FP8_BLOCK k % 16. */
+ * the _F8X2 codes quantize as their FP8 format).  k % 32; FP8_BLOCK k % 16,
+ * k <= 65536 and rows < 2^28. */
 int mx_fmt_quantize(mx_ctx* ctx, int wfmt, const float* w, int rows, int k, void* q,
                     void* scales);
 /* MLP with format weights: mpp_mlp_h_fp8e4m3_f_n128 / _h_fp8e5m2_f_n128 /

@@ -1030,6 +1030,8 @@ int mx_fmt_quantize(mx_ctx* c, int wfmt, const float* w, int rows, int k, void* 
   if (!w || !q || !scales || !aligned16(w) || !aligned16(q))
     return set_err(c, MX_EINVAL, "format quantize buffers must be non-null and 16-byte aligned.");
   if (wfmt == MX_WFMT_FP8_BLOCK) {
+    if (rows >= mx::kMaxRows || k > mx::kMaxBlocks * mx::kQBlock)
+      return set_err(c, MX_EINVAL, "block FP8 quantize needs rows below %d and k at most %d.", mx::kMaxRows, mx::kMaxBlocks * mx::kQBlock);
     MX_HIP(c, mx::launch_block_quantize_weights(w, rows, k, static_cast<uint8_t*>(q), static_cast<float*>(scales), c->stream));
     return MX_OK;
   }

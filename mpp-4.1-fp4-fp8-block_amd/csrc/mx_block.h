@@ -13,6 +13,7 @@ namespace mx {
 constexpr int kQBlock = 128;         // values (of weights: rows too) of one block scale
 constexpr int kMaxBlocks = 512;       // blocks of K in one product
 constexpr int kMaxRows = 1 << 28;     // rows of a block-scaled matrix: a launch's grid holds 2^32 threads
+constexpr int kMaxHidden = 1 << 28;   // values of an exchanged row: their place is an int
 constexpr int kMaxDirect = 8192;      // values of a row that launch_block_direct quantizes
 constexpr int kMaxRouteExperts = 512;
 constexpr int kMaxRouteGroups = 64;

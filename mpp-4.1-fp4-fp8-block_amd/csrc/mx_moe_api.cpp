@@ -225,7 +225,8 @@ int mx_moe_dispatch(mx_ctx* c, int tokens, int topk, int experts, const int32_t*
   if (!x != !xs) return fail(c, MX_EINVAL, "dispatch takes both x and xs or neither.");
   if (x) {
     if (!is_float(dtype)) return fail(c, MX_EINVAL, "dispatch rows must be f32, f16 or bf16.");
-    if (hidden < 1) return fail(c, MX_EINVAL, "dispatch hidden must be positive.");
+    if (hidden < 1 || hidden >= mx::kMaxHidden)
+      return fail(c, MX_EINVAL, "dispatch hidden must be positive and below %d.", mx::kMaxHidden);
     if (!is_aligned(x, size_of(dtype)) || !is_aligned(xs, size_of(dtype)))
       return fail(c, MX_EINVAL, "dispatch rows must be aligned to their elements.");
   }
@@ -248,7 +249,8 @@ int mx_moe_combine(mx_ctx* c, int tokens, int topk, int hidden, const void* y, i
                    const float* weights, const void* add, void* out, int out_dtype) {
   if (!c) return MX_EINVAL;
   if (int rc = check_slots(c, tokens, topk)) return rc;
-  if (hidden < 1) return fail(c, MX_EINVAL, "combine hidden must be positive.");
+  if (hidden < 1 || hidden >= mx::kMaxHidden)
+    return fail(c, MX_EINVAL, "combine hidden must be positive and below %d.", mx::kMaxHidden);
   if (!is_float(y_dtype) || !is_float(out_dtype)) return fail(c, MX_EINVAL, "combine rows must be f32, f16 or bf16.");
   if (tokens == 0) return MX_OK;
   if (!y || !rows || !weights || !out) return fail(c, MX_EINVAL, "combine buffers must not be null.");

@@ -54,3 +54,29 @@ def test_rows_past_a_grid_are_refused(dev):
     q = M.QMatrix(p.value, p.value)
     cfg, w = M.MlpConfig(1 << 28, 16, 16), M.MlpWeights(q, q, q)
     assert L.mx_fmt_mlp_forward(c, M.WFMT_FP8_BLOCK, ctypes.byref(cfg), p, ctypes.byref(w), p) == M.MX_EINVAL
+
+
+def test_sizes_past_an_int_are_refused(dev):
+    L, c, p = M.load(), dev.ctx, dev.alloc(4096).p
+    for hidden in (1 << 28, 0x7fffffff):
+        assert L.mx_moe_dispatch(c, 1, 1, 1, p, p, p, p, H, hidden, p) == M.MX_EINVAL
+        assert L.mx_moe_combine(c, 1, 1, hidden, p, H, p, p, None, p, H) == M.MX_EINVAL
+    assert L.mx_fmt_quantize(c, M.WFMT_FP8_BLOCK, p, 1 << 28, 16, p, p) == M.MX_EINVAL
+    assert L.mx_fmt_quantize(c, M.WFMT_FP8_BLOCK, p, 0x7fffffff, 16, p, p) == M.MX_EINVAL
+    assert L.mx_fmt_quantize(c, M.WFMT_FP8_BLOCK, p, 1, 65552, p, p) == M.MX_EINVAL
+
+
+def test_one_long_row(dev):
+    """The longest row of a token out and back."""
+    hidden = (1 << 28) - 1
+    x = dev.alloc(2 * hidden)
+    xs, out = dev.alloc(2 * hidden), dev.alloc(2 * hidden)
+    dev.fill_normal(x, H, hidden, seed=3)
+    dev.memset(out, 0)
+    ids, counts, rows, w = dev.upload(np.zeros(1, np.int32)), dev.alloc(4), dev.alloc(4), dev.upload(np.ones(1, np.float32))
+    dev.moe_dispatch(1, 1, 1, ids, counts, rows, x, H, hidden, xs)
+    dev.moe_combine(1, 1, hidden, xs, H, rows, w, out, H)
+    got, want = dev.download(out, np.float16, hidden), dev.download(x, np.float16, hidden)
+    for b in (x, xs, out):
+        b.free()
+    assert np.array_equal(got, want)
